@@ -322,9 +322,9 @@ def plain_cuts(logits, mask, p):
     under = (mass < p["top_p"][:, None].double() * mass.gather(1, last)).sum(1) + 1
     n = torch.where(p["top_p"] < 1, torch.minimum(n, under), n)
     last = (n - 1).clamp(min=0)[:, None]
-    none = n == 0
+    none, whole = n == 0, n == there.sum(1)  # (where nothing is cut off, the cut lies below every logit)
     return dict(total=torch.where(none, 0.0, mass.gather(1, last)[:, 0]), max=top[:, 0], temperature=torch.where(greedy, 0.0, p["temperature"]),
-                cut=torch.where(none, math.inf, x.gather(1, last)[:, 0]), cut_token=torch.where(none, -1, ids.gather(1, last)[:, 0]).to(torch.int32),
+                cut=torch.where(whole, -math.inf, x.gather(1, last)[:, 0]), cut_token=torch.where(whole, -1, ids.gather(1, last)[:, 0]).to(torch.int32),
                 n_kept=n.to(torch.int32), top_token=torch.where(none, -1, ids[:, 0]).to(torch.int32))
 
 
@@ -558,15 +558,15 @@ def exact_weights(x, mask, t):
 
 
 def exact_cut(x, mask, temperature, top_k, top_p, min_p):
-    """One row's kept tokens in falling order, their weights, and the rank of the row's tokens by (logit, token)."""
+    """(one row's kept tokens in falling order, all tokens' weights, whether tokens were cut off)."""
     w, x = exact_weights(x[None], mask if mask is None else mask[None], torch.tensor([temperature if temperature > 0 else 1.0], dtype=torch.float64, device=x.device))
     w, x = w[0], x[0]
     order = torch.argsort(x, descending=True, stable=True)
     order = order[:int(torch.isfinite(x).sum())]
     if not len(order):
-        return order, w
+        return order, w, False
     if not temperature > 0:
-        return order[:1], w
+        return order[:1], w, len(order) > 1
     keep = len(order)
     if min_p > 0:
         keep = max(1, int((w >= min_p).sum()))
@@ -575,7 +575,7 @@ def exact_cut(x, mask, temperature, top_k, top_p, min_p):
     if top_p < 1:
         run_ = torch.cumsum(w[order[:keep]], 0)
         keep = min(keep, int(torch.searchsorted(run_, (top_p * run_[-1]).view(1))) + 1)
-    return order[:keep], w
+    return order[:keep], w, keep < len(order)
 
 
 def exact(case, seed):
@@ -588,19 +588,15 @@ def exact(case, seed):
         probs = torch.zeros(case["rows"], case["vocab"], dtype=torch.float64, device="cuda") if case["probs"] else None
         for r in range(case["rows"]):
             x = s["logits"][r, :case["vocab"]]
-            kept, w = exact_cut(x, None if s["mask"] is None else s["mask"][r], p["temperature"][r], int(p["top_k"][r]), p["top_p"][r], p["min_p"][r])
+            kept, w, off = exact_cut(x, None if s["mask"] is None else s["mask"][r], p["temperature"][r], int(p["top_k"][r]), p["top_p"][r], p["min_p"][r])
             total = w[kept].sum()
             t = max(p["temperature"][r], 0.0)
-            if len(kept):
-                values = torch.stack([total, x[kept[0]].double().clamp(max=FLT_MAX), torch.tensor(t, dtype=torch.float64, device="cuda"),
-                                      x[kept[-1]].double().clamp(max=FLT_MAX), kept[-1].double(), torch.tensor(float(len(kept)), dtype=torch.float64, device="cuda"),
-                                      kept[0].double()])
-            else:
-                values = torch.tensor([0.0, -math.inf, t, math.inf, -1, 0, -1], dtype=torch.float64, device="cuda")
-            found.append(values)
+            last = (float(x[kept[-1]].double().clamp(max=FLT_MAX)), int(kept[-1])) if off else (-math.inf, -1)
+            first = (float(x[kept[0]].double().clamp(max=FLT_MAX)), int(kept[0])) if len(kept) else (-math.inf, -1)
+            found.append([float(total), first[0], t, *last, len(kept), first[1]])
             if probs is not None and len(kept):
                 probs[r, kept] = w[kept] / total
-        f = torch.stack(found, 1)
+        f = torch.tensor(found, dtype=torch.float64).T
         out = dict(total=f[0], max=f[1], temperature=f[2], cut=f[3], cut_token=f[4].to(torch.int32), n_kept=f[5].to(torch.int32), top_token=f[6].to(torch.int32))
         if probs is not None:
             out["probs"] = probs
