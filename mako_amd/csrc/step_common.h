@@ -1,0 +1,244 @@
+// What the kernels of a speculative decode step share: rows of logits of three types, weights in 64 bits, the order of a
+// row's tokens, and a workgroup's reductions and scans.  (The entry points: mako_step.hip.)
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/mako_step.h"
+
+extern "C" __device__ uint32_t __ockl_wfred_add_u32(uint32_t);
+extern "C" __device__ uint32_t __ockl_wfred_min_u32(uint32_t);
+extern "C" __device__ uint32_t __ockl_wfred_max_u32(uint32_t);
+extern "C" __device__ float __ockl_wfred_max_f32(float);
+extern "C" __device__ double __ockl_wfred_add_f64(double);
+extern "C" __device__ double __ockl_wfscan_add_f64(double, bool inclusive);
+extern "C" __device__ uint64_t __ockl_wfscan_add_u64(uint64_t, bool inclusive);
+
+namespace mako {
+namespace step {
+
+constexpr uint32_t kChunk = 1024;       // logits of a row that one wave takes: 16 a lane
+constexpr uint32_t kSlice = 4096;       // ... that a workgroup of 256 threads takes
+constexpr uint32_t kNoToken = 0xffffffffu;
+constexpr float kFltMax = 3.402823466e+38f;
+constexpr double kLog2e = 1.4426950408889634;
+
+// ---- types of logits: kVec of them are the 16 bytes that a lane loads at once ----
+// (a row may begin at any element: the loads promise no more than that)
+typedef uint32_t words_at_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t words_at_2 __attribute__((ext_vector_type(4), aligned(2)));
+struct F32 {
+    using raw = uint32_t;
+    using words = words_at_4;
+    static constexpr uint32_t kVec = 4;
+    static __device__ __forceinline__ float of(uint32_t w, int) { return __uint_as_float(w); }
+};
+struct BF16 {
+    using raw = uint16_t;
+    using words = words_at_2;
+    static constexpr uint32_t kVec = 8;
+    static __device__ __forceinline__ float of(uint32_t w, int k) { return __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16); }
+};
+struct F16 {
+    using raw = uint16_t;
+    using words = words_at_2;
+    static constexpr uint32_t kVec = 8;
+    static __device__ __forceinline__ float of(uint32_t w, int k)
+    {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(k & 1 ? w >> 16 : w));
+    }
+};
+
+// Logits i .. i + kVec - 1 of a row of n, as fp32; those at n and behind are NaN (no token).
+template <class E>
+__device__ __forceinline__ void load_vec(const void* row, uint32_t i, uint32_t n, float* x)
+{
+    using raw = typename E::raw;
+    const raw* p = static_cast<const raw*>(row) + i;
+    if (i + E::kVec <= n) {
+        const typename E::words w = *reinterpret_cast<const typename E::words*>(p);
+#pragma unroll
+        for (uint32_t k = 0; k < E::kVec; ++k)
+            x[k] = E::of(sizeof(raw) == 4 ? w[k % 4] : w[k / 2], (int)k);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < E::kVec; ++k) {
+            x[k] = __uint_as_float(0x7fc00000u);
+            if (i + k < n)
+                x[k] = E::of(p[k], 0);
+        }
+    }
+}
+
+// A logit as the operators see it: -inf for what is no token (masked, NaN, -inf), +inf as the largest finite value, and
+// -0 as 0 (the two are equal, and are one value to order_key()).
+__device__ __forceinline__ float token_logit(float x, bool allowed)
+{
+    return allowed && x > -INFINITY ? fminf(x, kFltMax) + 0.0f : -INFINITY;
+}
+
+template <class E>
+__device__ __forceinline__ void load_tokens(const void* row, const uint32_t* mask, uint32_t i, uint32_t n, float* x)
+{
+    load_vec<E>(row, i, n, x);
+    uint32_t bits = 0xffffffffu;
+    if (mask) // (i is a multiple of kVec: the vector's bits lie in one word)
+        bits = i < n ? mask[i >> 5] >> (i & 31u) : 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < E::kVec; ++k)
+        x[k] = token_logit(x[k], (bits >> k) & 1u);
+}
+
+// Rising keys are falling logits.
+__device__ __forceinline__ uint32_t order_key(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? u : ~(u | 0x80000000u);
+}
+__device__ __forceinline__ float key_logit(uint32_t k)
+{
+    return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
+}
+
+// 2^t for t <= 0: 2^round(t) times a polynomial in the rest, of degree 10 and constant term 1, the one whose largest
+// relative error over [-1/2, 1/2] is least (2.1e-16, found by exchange).  2^0 is exactly 1.  0 below 2^-1074.
+__device__ __forceinline__ double exp2_down(double t)
+{
+    t = fmax(t, -1100.0);
+    const double n = rint(t), f = t - n;
+    double p = 7.0372784767444307e-09;
+    p = fma(p, f, 1.020853789089708e-07);
+    p = fma(p, f, 1.3215662838949978e-06);
+    p = fma(p, f, 1.5252658116637374e-05);
+    p = fma(p, f, 0.00015403529961119085);
+    p = fma(p, f, 0.0013333558228561327);
+    p = fma(p, f, 0.0096181291080346051);
+    p = fma(p, f, 0.055504108664458832);
+    p = fma(p, f, 0.24022650695908768);
+    p = fma(p, f, 0.69314718055994973);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+
+// log2(e) / T, for weights 2^((x - max) scale).  (T infinite: as good as 0, but 0 times an infinity would be no number.)
+__device__ __forceinline__ double weight_scale(float temperature)
+{
+    return temperature > 0.0f ? fmax(kLog2e / (double)temperature, 1e-300) : 1e-300;
+}
+// (the difference first: it is exactly 0 for the largest logit, whose weight is exactly 1)
+__device__ __forceinline__ double weight(float x, double max_logit, double scale)
+{
+    return exp2_down(((double)x - max_logit) * scale);
+}
+
+__device__ __forceinline__ int lane()
+{
+    return threadIdx.x & 63;
+}
+__device__ __forceinline__ int wave()
+{
+    return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+}
+
+// ---- of a workgroup of W waves; every thread gets the result, and `s` may be used again at once ----
+template <int W>
+struct Share {
+    unsigned long long u[W];
+    double d[W];
+};
+
+template <int W>
+__device__ __forceinline__ uint32_t all_sum(uint32_t v, Share<W>& s)
+{
+    v = __ockl_wfred_add_u32(v);
+    if (lane() == 0)
+        s.u[wave()] = v;
+    __syncthreads();
+    uint32_t t = 0;
+    for (int w = 0; w < W; ++w)
+        t += (uint32_t)s.u[w];
+    __syncthreads();
+    return t;
+}
+template <int W>
+__device__ __forceinline__ uint32_t all_min(uint32_t v, Share<W>& s)
+{
+    v = __ockl_wfred_min_u32(v);
+    if (lane() == 0)
+        s.u[wave()] = v;
+    __syncthreads();
+    uint32_t t = 0xffffffffu;
+    for (int w = 0; w < W; ++w)
+        t = min(t, (uint32_t)s.u[w]);
+    __syncthreads();
+    return t;
+}
+template <int W>
+__device__ __forceinline__ float all_max(float v, Share<W>& s)
+{
+    v = __ockl_wfred_max_f32(v);
+    if (lane() == 0)
+        s.d[wave()] = (double)v;
+    __syncthreads();
+    float t = -INFINITY;
+    for (int w = 0; w < W; ++w)
+        t = fmaxf(t, (float)s.d[w]);
+    __syncthreads();
+    return t;
+}
+// (in a fixed order: the lanes of a wave, then the waves)
+template <int W>
+__device__ __forceinline__ double all_sum(double v, Share<W>& s)
+{
+    v = __ockl_wfred_add_f64(v);
+    if (lane() == 0)
+        s.d[wave()] = v;
+    __syncthreads();
+    double t = 0.0;
+    for (int w = 0; w < W; ++w)
+        t += s.d[w];
+    __syncthreads();
+    return t;
+}
+// What the threads before this one have; `total`: what all have.
+template <int W>
+__device__ __forceinline__ double sum_before(double v, double& total, Share<W>& s)
+{
+    const double mine = __ockl_wfscan_add_f64(v, true);
+    if (lane() == 63)
+        s.d[wave()] = mine;
+    __syncthreads();
+    double before = 0.0, t = 0.0;
+    for (int w = 0; w < W; ++w) {
+        if (w == wave())
+            before = t;
+        t += s.d[w];
+    }
+    __syncthreads();
+    total = t;
+    // (not mine - v, which rounds: what the lane before has)
+    const double left = __shfl_up(mine, 1);
+    return before + (lane() ? left : 0.0);
+}
+template <int W>
+__device__ __forceinline__ unsigned long long sum_before(unsigned long long v, unsigned long long& total, Share<W>& s)
+{
+    const unsigned long long mine = __ockl_wfscan_add_u64(v, true);
+    if (lane() == 63)
+        s.u[wave()] = mine;
+    __syncthreads();
+    unsigned long long before = 0, t = 0;
+    for (int w = 0; w < W; ++w) {
+        if (w == wave())
+            before = t;
+        t += s.u[w];
+    }
+    __syncthreads();
+    total = t;
+    return before + mine - v;
+}
+
+} // namespace step
+} // namespace mako
