@@ -9,7 +9,7 @@ CSRC = os.path.join(HERE, "csrc")
 # which other kernels exist; they also compile side by side)
 SOURCES = ["mako_sampler.hip", "k_scan.hip", "k_finish.hip", "k_finish_halves.hip", "k_plan_alone.hip", "k_sort.hip", "k_sort_unsorted.hip", "k_tail.hip", "k_tail_unsorted.hip", "k_index.hip",
            "k_beside_finish.hip", "k_beside_sort.hip", "k_beside_tail.hip",
-           "mako_step.hip", "k_step_cut.hip", "k_step_verify.hip", "k_step_blocks.hip"]
+           "mako_step.hip", "k_step_scan.hip", "k_step_cut.hip", "k_step_verify.hip", "k_step_blocks.hip"]
 OBJ_DIR = os.path.join(HERE, "csrc", "_obj")
 OUT = os.path.join(HERE, "libmako_sampler.so")
 # the same library with the kernels' index checks compiled in (-DMAKO_CHECKED): for the test that runs the workloads

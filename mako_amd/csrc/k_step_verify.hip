@@ -1,6 +1,6 @@
 // Verification of drafted tokens (mako_step_verify_drafts).
 //
-//   left_kernel  a workgroup for every slice of 4096 tokens of every request: where the request stops accepting, and what
+//   left_kernel  a workgroup for every part of 4096 tokens of every request: where the request stops accepting, and what
 //                the slice has left there to draw from
 //   draw_kernel  a workgroup for every request: the slice that the uniform falls into, and the token in it
 #include "step_common.h"
@@ -11,7 +11,7 @@ namespace step {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr uint32_t kRun = 8, kRuns = kSlice / kThreads / kRun; // a thread has runs of 8 tokens: of either row, whatever its type
+constexpr uint32_t kRun = 8, kRuns = kPart / kThreads / kRun; // a thread has runs of 8 tokens: of either row, whatever its type
 
 // A row of weights: logits under their cut, or probabilities.
 template <class E>
@@ -102,7 +102,7 @@ struct Left {
         double sum = 0.0;
 #pragma unroll
         for (uint32_t j = 0; j < kRuns; ++j)
-            run(s * kSlice + (j * kThreads + threadIdx.x) * kRun, r + j * kRun);
+            run(s * kPart + (j * kThreads + threadIdx.x) * kRun, r + j * kRun);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             sum += r[k];
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) left_kernel(mako_verify_desc d, Scra
     double r[16];
     const double sum = all_sum<kWaves>(left.slice(blockIdx.x, r), share);
     if (threadIdx.x == 0) {
-        sc.parts[(uint64_t)b * sc.slices_cap + blockIdx.x] = sum;
+        sc.parts[(uint64_t)b * sc.parts_cap + blockIdx.x] = sum;
         if (blockIdx.x == 0)
             sc.stop[b] = accepted;
     }
@@ -188,8 +188,8 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
         return;
     const uint32_t accepted = sc.stop[b];
     Left<E, Q> left = left_of<E, Q>(d, b, accepted, drafts);
-    const uint32_t slices = (d.n_vocab + kSlice - 1) / kSlice;
-    double* parts = sc.parts + (uint64_t)b * sc.slices_cap;
+    const uint32_t slices = (d.n_vocab + kPart - 1) / kPart;
+    double* parts = sc.parts + (uint64_t)b * sc.parts_cap;
     double r[16];
     // the slices: one to a thread (no more than 256 of them)
     double part = threadIdx.x < slices ? parts[threadIdx.x] : 0.0, total;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
         uint32_t hit = kNoToken, weighty = 0; // (weighty: a token + 1)
 #pragma unroll
         for (uint32_t j = 0; j < kRuns; ++j) {
-            const uint32_t i = at * kSlice + (j * kThreads + threadIdx.x) * kRun;
+            const uint32_t i = at * kPart + (j * kThreads + threadIdx.x) * kRun;
             double mine = 0.0, all;
 #pragma unroll
             for (uint32_t k = 0; k < kRun; ++k)
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
 template <class E, class Q>
 void verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
 {
-    hipLaunchKernelGGL((left_kernel<E, Q>), dim3((d.n_vocab + kSlice - 1) / kSlice, d.n_requests), dim3(kThreads), 0, st, d, sc);
+    hipLaunchKernelGGL((left_kernel<E, Q>), dim3((d.n_vocab + kPart - 1) / kPart, d.n_requests), dim3(kThreads), 0, st, d, sc);
     hipLaunchKernelGGL((draw_kernel<E, Q>), dim3(d.n_requests), dim3(kThreads), 0, st, d, sc);
 }
 template <class E>

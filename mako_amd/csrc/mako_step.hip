@@ -81,14 +81,16 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     ctx->max_vocab = max_vocab;
     const OnDevice on(device);
     mako::step::Scratch& sc = ctx->sc;
-    sc.chunks_cap = (max_vocab + mako::step::kChunk - 1) / mako::step::kChunk;
-    sc.slices_cap = (max_vocab + mako::step::kSlice - 1) / mako::step::kSlice;
+    sc.chunks_cap = mako::step::chunks_of(max_vocab);
+    sc.parts_cap = (max_vocab + mako::step::kPart - 1) / mako::step::kPart;
     const uint64_t rows = max_rows;
     hipError_t e = on.status();
     if (e == hipSuccess)
         e = take(sc.chunks, rows * sc.chunks_cap);
     if (e == hipSuccess)
-        e = take(sc.parts, rows * sc.slices_cap);
+        e = take(sc.lists, rows * sc.chunks_cap * mako::step::kChunkList);
+    if (e == hipSuccess)
+        e = take(sc.parts, rows * sc.parts_cap);
     if (e == hipSuccess)
         e = take(sc.stop, rows);
     if (e == hipSuccess)
@@ -117,7 +119,7 @@ void mako_step_destroy(mako_step_ctx* ctx)
     {
         const OnDevice on(ctx->device);
         mako::step::Scratch& sc = ctx->sc;
-        void* ptrs[] = {sc.chunks, sc.parts, sc.stop, sc.released, sc.taken, sc.held, sc.free_state};
+        void* ptrs[] = {sc.chunks, sc.lists, sc.parts, sc.stop, sc.released, sc.taken, sc.held, sc.free_state};
         for (void* p : ptrs)
             if (p)
                 (void)hipFree(p);

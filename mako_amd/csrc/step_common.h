@@ -13,14 +13,14 @@ extern "C" __device__ uint32_t __ockl_wfred_min_u32(uint32_t);
 extern "C" __device__ uint32_t __ockl_wfred_max_u32(uint32_t);
 extern "C" __device__ float __ockl_wfred_max_f32(float);
 extern "C" __device__ double __ockl_wfred_add_f64(double);
+extern "C" __device__ uint32_t __ockl_wfscan_add_u32(uint32_t, bool inclusive);
 extern "C" __device__ double __ockl_wfscan_add_f64(double, bool inclusive);
 extern "C" __device__ uint64_t __ockl_wfscan_add_u64(uint64_t, bool inclusive);
 
 namespace mako {
 namespace step {
 
-constexpr uint32_t kChunk = 1024;       // logits of a row that one wave takes: 16 a lane
-constexpr uint32_t kSlice = 4096;       // ... that a workgroup of 256 threads takes
+constexpr uint32_t kPart = 4096;        // logits of a row that a workgroup of 256 threads takes: 16 a thread
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr float kFltMax = 3.402823466e+38f;
 constexpr double kLog2e = 1.4426950408889634;

@@ -9,26 +9,39 @@
 namespace mako {
 namespace step {
 
-// What a wave finds in its chunk of a row.
+// A row is read in chunks of 1024 logits, a wave each.
+constexpr uint32_t kChunk = 1024;
+constexpr uint32_t kChunkList = 64; // a chunk's first tokens that are written out, at most
+
 struct ChunkRec {
-    double sum;     // of the weights, relative to the chunk's own largest logit
-    float max;      // -inf: no token
-    uint32_t count; // of tokens
+    double sum;      // of the weights, relative to the chunk's own largest logit (rows that need their total)
+    float max;       // -inf: no token
+    float listed;    // all tokens of this logit and above are in the list; +inf: none
+    uint32_t count;  // tokens
+    uint32_t n_list;
+    uint32_t first;  // the first token of the largest logit
+    float low;       // the smallest logit (rows with a min_p)
 };
 
-// Of a batch of requests: where a request stopped accepting, and what is left to draw from in each slice of that row.
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
+    uint64_t* lists;      // [rows][chunks_cap][kChunkList]: (order key, token)
     uint32_t chunks_cap;  // of a row
-    double* parts;        // [rows][slices_cap]
-    uint32_t slices_cap;
-    uint32_t* stop;       // [rows]
+    double* parts;        // [rows][parts_cap]: what is left to draw from in each part of the row where a request stops
+    uint32_t parts_cap;
+    uint32_t* stop;       // [rows] drafts a request accepts
     uint32_t* released;   // [rows + 1] blocks given back by the requests before
     uint32_t* taken;      // [rows + 1] blocks taken by the requests before
     uint32_t* held;       // [rows] blocks a request keeps before it takes any
     uint32_t* free_state; // [2] blocks on the free list before the call, and after the releases
 };
 
+__host__ __device__ inline uint32_t chunks_of(uint32_t n_vocab)
+{
+    return (n_vocab + kChunk - 1) / kChunk;
+}
+
+void launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
 void launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
 void launch_probs(hipStream_t st, const mako_cut_desc& d);
 void launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc);
