@@ -13,6 +13,8 @@ namespace step {
 constexpr uint32_t kChunk = 1024;
 constexpr uint32_t kChunkList = 64; // a chunk's first tokens that are written out, at most
 
+// (what the second pass over a row, around its cut, finds in a chunk takes the same place: `sum` of the tokens that are weighed,
+// `count` of those above, `n_list` in the list)
 struct ChunkRec {
     double sum;      // of the weights, relative to the chunk's own largest logit (rows that need their total)
     float max;       // -inf: no token
@@ -23,10 +25,22 @@ struct ChunkRec {
     float low;       // the smallest logit (rows with a min_p)
 };
 
+// A row whose cut lies further down than the chunks' lists: what the second pass looks for.
+struct RowPlan {
+    double mass, total; // the cut is behind the first tokens that weigh `mass`, of all that weigh `total` (0: not known),
+    uint32_t rank;      // or, if not 0, behind the first `rank`
+    uint32_t tokens;    // of the row
+    float low, high;    // the tokens from `low` up to `high` are listed,
+    uint32_t from_above; // those above are weighed, or those below
+    uint32_t look;       // 0: there is no guess where it lies
+};
+
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
     uint64_t* lists;      // [rows][chunks_cap][kChunkList]: (order key, token)
     uint32_t chunks_cap;  // of a row
+    RowPlan* plans;       // [rows]
+    uint32_t* wide;       // [rows + 1]: how many rows have a plan, and which
     double* parts;        // [rows][parts_cap]: what is left to draw from in each part of the row where a request stops
     uint32_t parts_cap;
     uint32_t* stop;       // [rows] drafts a request accepts
@@ -42,6 +56,7 @@ __host__ __device__ inline uint32_t chunks_of(uint32_t n_vocab)
 }
 
 void launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
+void launch_look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
 void launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
 void launch_probs(hipStream_t st, const mako_cut_desc& d);
 void launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc);
