@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr uint32_t kBins = 1024;  // two to a thread
-constexpr uint32_t kList = 6144;  // tokens that are held in LDS
+constexpr uint32_t kList = kWholeRow; // tokens that are held in LDS
 constexpr uint32_t kSmall = 1024; // ... of a bin
 constexpr uint32_t kCrowd = 256;  // ... that are counted against each other
 static_assert(kBins == 2 * kThreads, "two bins to a thread");
@@ -32,7 +32,7 @@ struct RowLds {
     uint32_t count[kBins];
     Share<kWaves> share;
     uint32_t counts[kWaves];
-    uint32_t n, at, before, id;
+    uint32_t n, at, before, id, first;
     u64 mass_before;
     double m;
 };
@@ -458,7 +458,7 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
 }
 
 // A row's chunks together: every wave does it by itself, a lane for every 64th chunk.
-constexpr uint32_t kHeld = 4; // of a lane's chunks that are in registers
+constexpr uint32_t kHeld = 2; // of a lane's chunks that are in registers
 struct Chunks {
     ChunkRec rec[kHeld];
     float max, listed, low;
@@ -514,77 +514,84 @@ struct Chunks {
     }
 };
 
-// The chunks' lists, half a wave to a chunk: the first 32 tokens of those in registers are asked for together with the chunks'
-// records, whatever their number is.
-constexpr uint32_t kPairs = 32 / kWaves; // of 64 chunks, by a wave
+// The chunks' lists, kSlots lanes to a chunk: their first kSlots tokens, of as many chunks as fit kAhead loads, are asked for
+// together with the chunks' records, whatever their number is.
+template <uint32_t kSlots, uint32_t kRoom, uint32_t kAhead>
 struct Lists {
-    uint64_t entry[kHeld][kPairs];
+    static constexpr uint32_t kOfWave = 64 / kSlots, kOfAll = kOfWave * kWaves; // chunks of a load
+    static_assert(kOfAll <= 64 && kAhead * kOfAll <= kHeld * 64u, "chunks that are in registers");
+    uint64_t entry[kAhead];
 
-    static __device__ __forceinline__ uint32_t chunk(uint32_t h, uint32_t q) { return h * 64u + (q * kWaves + (uint32_t)wave()) * 2u + (uint32_t)lane() / 32u; }
+    static __device__ __forceinline__ uint32_t chunk(uint32_t a) { return a * kOfAll + (uint32_t)wave() * kOfWave + (uint32_t)lane() / kSlots; }
 
     __device__ __forceinline__ void load(const uint64_t* lists, uint32_t chunks)
     {
 #pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h)
-#pragma unroll
-            for (uint32_t q = 0; q < kPairs; ++q) {
-                entry[h][q] = ~0ull;
-                if (chunk(h, q) < chunks)
-                    entry[h][q] = lists[chunk(h, q) * kChunkList + (uint32_t)lane() % 32u];
-            }
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            entry[a] = 0;
+            if (chunk(a) < chunks)
+                entry[a] = lists[chunk(a) * kRoom + (uint32_t)lane() % kSlots];
+        }
     }
-    // Those up to `key` into lds.list (lds.n is 0); how many there are, which may be more than there is room for.
-    __device__ __forceinline__ uint32_t gather(const Chunks& c, const ChunkRec* recs, const uint64_t* lists, uint32_t chunks, uint32_t key, RowLds& lds) const
+    // The tokens of logits from `from` on into lds.list (lds.n is 0), and the first of those of logit `max` into lds.first; how
+    // many there are, which may be more than there is room for.
+    __device__ __forceinline__ uint32_t gather(const Chunks& c, const ChunkRec* recs, const uint64_t* lists, uint32_t chunks, float from, float max, RowLds& lds) const
     {
         const u64 before = (1ull << lane()) - 1ull;
-        u64 in[kHeld][kPairs];
+        auto put = [&](uint64_t e, bool in, uint32_t place) {
+            const float x = __uint_as_float((uint32_t)(e >> 32));
+            if (in && x == max)
+                atomicMin(&lds.first, (uint32_t)e);
+            if (in && place < kList)
+                lds.list[place] = (uint64_t)order_key(x + 0.0f) << 32 | (uint32_t)e;
+        };
+        u64 in[kAhead];
         uint32_t n = 0, longest = 0;
 #pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h) {
-            longest = max(longest, c.rec[h].n_list);
+        for (uint32_t h = 0; h < kHeld; ++h)
+            longest = ::max(longest, c.rec[h].n_list);
 #pragma unroll
-            for (uint32_t q = 0; q < kPairs; ++q) {
-                const uint32_t of_chunk = (uint32_t)__shfl((int)c.rec[h].n_list, (int)(chunk(h, q) & 63u));
-                in[h][q] = __ballot((uint32_t)lane() % 32u < of_chunk && (uint32_t)(entry[h][q] >> 32) <= key);
-                n += (uint32_t)__popcll(in[h][q]);
-            }
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t of_chunk = (uint32_t)__shfl((int)c.rec[a * kOfAll / 64u].n_list, (int)(chunk(a) & 63u));
+            in[a] = __ballot(chunk(a) < chunks && (uint32_t)lane() % kSlots < of_chunk && __uint_as_float((uint32_t)(entry[a] >> 32)) >= from);
+            n += (uint32_t)__popcll(in[a]);
         }
         uint32_t at = 0;
         if (lane() == 0 && n)
             at = atomicAdd(&lds.n, n);
         at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
 #pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h)
-#pragma unroll
-            for (uint32_t q = 0; q < kPairs; ++q) {
-                const uint32_t place = at + (uint32_t)__popcll(in[h][q] & before);
-                if ((in[h][q] >> lane() & 1ull) && place < kList)
-                    lds.list[place] = entry[h][q];
-                at += (uint32_t)__popcll(in[h][q]);
-            }
+        for (uint32_t a = 0; a < kAhead; ++a) {
+            put(entry[a], in[a] >> lane() & 1ull, at + (uint32_t)__popcll(in[a] & before));
+            at += (uint32_t)__popcll(in[a]);
+        }
         // longer lists, and the chunks beyond
-        auto rest = [&](uint32_t i, uint32_t from) {
+        auto rest = [&](uint32_t i, uint32_t slot) {
             const uint32_t of_chunk = recs[i].n_list;
-            const uint64_t e = from + (uint32_t)lane() < of_chunk ? lists[i * kChunkList + from + (uint32_t)lane()] : ~0ull;
-            const u64 more = __ballot(from + (uint32_t)lane() < of_chunk && (uint32_t)(e >> 32) <= key);
-            if (more) {
+            for (; slot < of_chunk; slot += 64u) {
+                const uint64_t e = slot + (uint32_t)lane() < of_chunk ? lists[i * kRoom + slot + (uint32_t)lane()] : 0ull;
+                const bool in_list = slot + (uint32_t)lane() < of_chunk && __uint_as_float((uint32_t)(e >> 32)) >= from;
+                const u64 more = __ballot(in_list);
                 uint32_t to = 0;
-                if (lane() == 0)
+                if (lane() == 0 && more)
                     to = atomicAdd(&lds.n, (uint32_t)__popcll(more));
-                to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to) + (uint32_t)__popcll(more & before);
-                if ((more >> lane() & 1ull) && to < kList)
-                    lds.list[to] = e;
+                to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
+                put(e, in_list, to + (uint32_t)__popcll(more & before));
             }
         };
-        if (__ballot(longest > 32u))
-            for (uint32_t i = (uint32_t)wave(); i < min(chunks, kHeld * 64u); i += kWaves)
-                rest(i, 32u);
-        for (uint32_t i = kHeld * 64u + (uint32_t)wave(); i < chunks; i += kWaves)
+        if (__ballot(longest > kSlots))
+            for (uint32_t i = (uint32_t)wave(); i < min(chunks, kAhead * kOfAll); i += kWaves)
+                rest(i, kSlots);
+        for (uint32_t i = kAhead * kOfAll + (uint32_t)wave(); i < chunks; i += kWaves)
             rest(i, 0u);
         __syncthreads();
-        return lds.n;
+        const uint32_t all = lds.n;
+        __syncthreads();
+        return all;
     }
 };
+using FirstLists = Lists<32, kChunkList, 5>; // (80 chunks: vocabularies of up to 163 840)
+using LookLists = Lists<64, kLookList, 10>;
 
 __device__ __forceinline__ void store_cut(mako_row_cut& out, const Cut& cut, uint32_t tokens)
 {
@@ -610,14 +617,42 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     c.load(recs, chunks);
     const mako_sampling_params p = d.params[r / d.rows_per_params];
     const RowKind kind(p);
-    Lists listed;
+    FirstLists listed;
+    const bool whole = d.n_vocab <= kWholeRow;
     if (kind.cut) {
-        listed.load(lists, chunks);
+        if (!whole)
+            listed.load(lists, chunks);
         clear_bins(lds);
-        if (threadIdx.x == 0)
+        if (threadIdx.x == 0) {
             lds.n = 0;
+            lds.first = kNoToken;
+        }
     }
     c.join(recs, chunks, kind);
+    Row<E> row(d, r, c.max, kind.scale);
+    uint32_t first = c.first, n_listed = 0;
+    if (kind.cut && c.count) {
+        __syncthreads();
+        if (whole) {
+            row.each([&](uint32_t id, float v) { lds.list[atomicAdd(&lds.n, 1u)] = (uint64_t)order_key(v) << 32 | id; });
+            __syncthreads();
+            n_listed = c.count;
+            c.listed = -INFINITY;
+        } else {
+            if (c.listed < INFINITY)
+                n_listed = listed.gather(c, recs, lists, chunks, c.listed, c.max, lds);
+            first = lds.first;
+            if (first == kNoToken) { // (too many equal ones for any list)
+                __syncthreads();
+                row.each([&](uint32_t id, float v) {
+                    if (v == c.max)
+                        atomicMin(&lds.first, id);
+                });
+                __syncthreads();
+                first = lds.first;
+            }
+        }
+    }
     mako_row_cut& out = d.out_cuts[r];
     if (threadIdx.x == 0) {
         mako_row_cut plain;
@@ -625,18 +660,13 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         plain.max_logit = c.max;
         plain.temperature = kind.greedy ? 0.0f : p.temperature;
         plain.n_kept = kind.greedy ? min(c.count, 1u) : c.count;
-        plain.top_token = (int32_t)c.first;
+        plain.top_token = (int32_t)first;
         plain.cut_logit = plain.n_kept < c.count ? c.max : -INFINITY;
         plain.cut_token = plain.n_kept < c.count ? plain.top_token : -1;
         out = plain;
     }
     if (!kind.cut || c.count == 0)
         return;
-    Row<E> row(d, r, c.max, kind.scale);
-    __syncthreads();
-    const uint32_t key = c.listed > -INFINITY ? order_key(c.listed + 0.0f) : 0xffffffffu;
-    const uint32_t n_listed = c.listed < INFINITY ? listed.gather(c, recs, lists, chunks, key, lds) : 0u;
-    __syncthreads();
     const bool list_there = n_listed > 0 && n_listed <= kList;
     // (weights' units: by the total, or, where it is not known, by the most that the list can weigh)
     row.set_unit(kind.sums ? c.total : (double)max(n_listed, 1u));
@@ -711,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
         const uint32_t r = sc.wide[1 + i];
         const RowPlan plan = sc.plans[r];
         const ChunkRec* recs = sc.chunks + (uint64_t)r * sc.chunks_cap;
-        const uint64_t* lists = sc.lists + (uint64_t)r * sc.chunks_cap * kChunkList;
+        const uint64_t* lists = sc.looks + (uint64_t)r * sc.chunks_cap * kLookList;
         const mako_sampling_params p = d.params[r / d.rows_per_params];
         const RowKind kind(p);
         mako_row_cut& out = d.out_cuts[r];
@@ -725,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             lds.n = 0;
         if (plan.look) {
             Chunks c;
-            Lists listed;
+            LookLists listed;
             c.load(recs, chunks);
             listed.load(lists, chunks);
             double side = 0.0;
@@ -734,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             auto add = [&](const ChunkRec& one) {
                 side += one.sum;
                 above += one.count;
-                room = room && one.n_list <= kChunkList;
+                room = room && one.n_list <= kLookList;
             };
 #pragma unroll
             for (uint32_t h = 0; h < kHeld; ++h)
@@ -746,8 +776,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             above = __ockl_wfred_add_u32(above);
             if (!__ballot(!room)) {
                 __syncthreads();
-                const uint32_t n = listed.gather(c, recs, lists, chunks, 0xffffffffu, lds);
-                __syncthreads();
+                const uint32_t n = listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
                 if (n > 0 && n <= kList) {
                     row.set_unit(kind.sums ? total : (double)kList);
                     const float from = fminf(plan.high, row.max);

@@ -25,11 +25,18 @@ __device__ __forceinline__ float nth_largest(float v, uint32_t n)
     return key_logit(~found);
 }
 
-// A chunk's logits, 16 to a lane; -inf: no token.
+constexpr int kEach = kChunk / 64; // logits of a lane
+
+__device__ __forceinline__ uint32_t lanes_before(unsigned long long lanes)
+{
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
+}
+
+// A chunk's logits; -inf: no token.
 template <class E>
 struct Chunk {
     uint32_t begin;
-    float x[16];
+    float x[kEach];
 
     // (the k-th logit's token)
     __device__ __forceinline__ uint32_t token(int k) const { return begin + ((uint32_t)k / E::kVec * 64u + (uint32_t)lane()) * E::kVec + (uint32_t)k % E::kVec; }
@@ -37,47 +44,47 @@ struct Chunk {
     __device__ __forceinline__ Chunk(const mako_cut_desc& d, uint32_t row, uint32_t chunk) : begin(chunk * kChunk)
     {
         const void* x_row = static_cast<const typename E::raw*>(d.logits) + (int64_t)row * d.logits_stride;
-        const uint32_t* mask = d.mask ? d.mask + (int64_t)row * d.mask_stride : nullptr;
+        if (begin + kChunk <= d.n_vocab) {
 #pragma unroll
-        for (int k = 0; k < 16; k += (int)E::kVec)
-            load_vec<E>(x_row, token(k), d.n_vocab, x + k);
+            for (int k = 0; k < kEach; k += (int)E::kVec)
+                load_whole<E>(x_row, token(k), x + k);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+            for (int k = 0; k < kEach; k += (int)E::kVec)
+                load_vec<E>(x_row, token(k), d.n_vocab, x + k);
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
             x[k] = fmaxf(x[k], -INFINITY); // (of a NaN and a number, the number)
-        if (mask) {
+        if (d.mask) {
+            const uint32_t* mask = d.mask + (int64_t)row * d.mask_stride;
 #pragma unroll
-            for (int k = 0; k < 16; k += (int)E::kVec) {
+            for (int k = 0; k < kEach; k += (int)E::kVec) {
                 const uint32_t i = token(k), bits = i < d.n_vocab ? mask[i >> 5] >> (i & 31u) : 0u;
 #pragma unroll
-                for (int e = 0; e < (int)E::kVec; ++e)
-                    if (!((bits >> e) & 1u))
-                        x[k + e] = -INFINITY;
+                for (int e = 0; e < (int)E::kVec; ++e) {
+                    const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - e)) >> 31);
+                    x[k + e] = __uint_as_float((__float_as_uint(x[k + e]) & keep) | (0xff800000u & ~keep));
+                }
             }
         }
     }
     __device__ __forceinline__ void no_infinity()
     {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+        for (int k = 0; k < kEach; ++k)
             x[k] = fminf(x[k], kFltMax);
     }
-    // The tokens of `in` (a bit for every lane's k-th) into a list.
-    __device__ __forceinline__ void list(const unsigned long long* in, uint64_t* to) const
+    // The lanes' k-th token, of those that have it `in` (the lanes `all`), into a list at `base`.
+    __device__ __forceinline__ void put(uint64_t* list, int k, bool in, unsigned long long all, uint32_t base) const
     {
-        const unsigned long long before = (1ull << lane()) - 1ull;
-        uint32_t base = 0;
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (in[k]) {
-                if (in[k] >> lane() & 1ull)
-                    to[base + (uint32_t)__popcll(in[k] & before)] = (uint64_t)order_key(x[k] + 0.0f) << 32 | token(k);
-                base += (uint32_t)__popcll(in[k]);
-            }
+        if (in)
+            list[base + lanes_before(all)] = (uint64_t)__float_as_uint(x[k]) << 32 | token(k);
     }
 };
 
 template <class E>
-__global__ void __launch_bounds__(256, 8) scan_kernel(mako_cut_desc d, Scratch sc)
+__global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch sc)
 {
     const uint32_t row = blockIdx.y, chunk = blockIdx.x * 4u + (uint32_t)wave(), chunks = chunks_of(d.n_vocab);
     if (row == 0 && chunk == 0 && lane() == 0)
@@ -85,81 +92,88 @@ __global__ void __launch_bounds__(256, 8) scan_kernel(mako_cut_desc d, Scratch s
     if (chunk >= chunks)
         return;
     Chunk<E> c(d, row, chunk);
-    float(&x)[16] = c.x;
+    const float(&x)[kEach] = c.x;
     const RowKind kind(d.params[row / d.rows_per_params]);
-    float mine = -INFINITY;
-    ChunkRec rec = {0.0, -INFINITY, -INFINITY, 0u, 0u, kNoToken, INFINITY};
+    float mine = x[0], low = x[0];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 1; k < kEach; ++k) {
         mine = fmaxf(mine, x[k]);
-        rec.count += (uint32_t)__popcll(__ballot(x[k] > -INFINITY));
+        low = fminf(low, x[k]);
     }
+    ChunkRec rec = {0.0, -INFINITY, -INFINITY, 0u, 0u, kNoToken, INFINITY};
     rec.max = __ockl_wfred_max_f32(mine);
     if (rec.max == INFINITY) {
         c.no_infinity();
         mine = fminf(mine, kFltMax);
         rec.max = kFltMax;
     }
+    const bool full = !__ballot(low == -INFINITY); // nothing but tokens
+    if (full) {
+        rec.count = kChunk;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            rec.count += (uint32_t)__popcll(__ballot(x[k] > -INFINITY));
+    }
     const uint64_t at = (uint64_t)row * sc.chunks_cap + chunk;
     if (rec.count) {
-        uint32_t id = kNoToken;
-        if (mine == rec.max) {
-#pragma unroll
-            for (int k = 15; k >= 0; --k)
-                id = x[k] == rec.max ? c.token(k) : id;
-        }
-        rec.first = __ockl_wfred_min_u32(id);
         if (kind.sums) {
             const double md = (double)rec.max;
-            // (weights below 2^-64 of the largest are nothing beside it)
-            if (rec.count > 1) {
-                double sum = 0.0;
+            double sum = 0.0;
+            // (eight at a time: all at once would not leave the logits in registers)
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    sum += weight(x[k], md, kind.scale);
-                rec.sum = __ockl_wfred_add_f64(sum);
-            } else {
-                rec.sum = 1.0;
+            for (int k = 0; k < kEach; ++k) {
+                sum += weight(x[k], md, kind.scale);
+                if (k % 8 == 7)
+                    __builtin_amdgcn_sched_barrier(0);
             }
+            rec.sum = __ockl_wfred_add_f64(sum);
         }
         if (kind.min_p) {
-            float low = INFINITY;
+            if (!full) {
+                low = INFINITY;
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-                low = fminf(low, x[k] > -INFINITY ? x[k] : INFINITY);
+                for (int k = 0; k < kEach; ++k)
+                    low = fminf(low, x[k] > -INFINITY ? x[k] : INFINITY);
+            }
             rec.low = -__ockl_wfred_max_f32(-low);
         }
-        if (kind.cut) {
+        if (kind.cut && d.n_vocab > kWholeRow) {
             // the chunk's first tokens: those not below the n-th largest of the lanes' largest; above it, where these are too
             // many (equal ones); none, where these are too many too.  A chunk of few tokens lists them all.
-            rec.listed = nth_largest(mine, kind.list_length(chunks));
-            unsigned long long in[16];
+            rec.listed = rec.count <= kChunkList ? -kFltMax : nth_largest(mine, kind.list_length(chunks));
+            uint64_t* list = sc.lists + at * kChunkList;
             auto take = [&](bool above) {
                 rec.n_list = 0;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    in[k] = __ballot(above ? x[k] > rec.listed : x[k] >= rec.listed);
-                    rec.n_list += (uint32_t)__popcll(in[k]);
+                for (int k = 0; k < kEach; ++k) {
+                    const bool in = above ? x[k] > rec.listed : x[k] >= rec.listed;
+                    const unsigned long long all = __ballot(in);
+                    if (all) {
+                        const uint32_t n = (uint32_t)__popcll(all);
+                        if (rec.n_list + n <= kChunkList)
+                            c.put(list, k, in, all, rec.n_list);
+                        rec.n_list += n;
+                    }
                 }
             };
-            if (rec.count <= kChunkList)
-                rec.listed = -kFltMax;
             take(false);
-            bool strict = false;
             if (rec.n_list > kChunkList) {
                 take(true);
-                strict = true;
+                rec.listed = key_logit(order_key(rec.listed + 0.0f) - 1u); // (all of the next larger number and above)
+                if (rec.n_list > kChunkList) {
+                    rec.n_list = 0;
+                    rec.listed = INFINITY;
+                }
             }
-            if (rec.n_list > kChunkList) {
-                rec.n_list = 0;
-                rec.listed = INFINITY;
-            } else {
-                c.list(in, sc.lists + at * kChunkList);
-                if (strict) // (the next larger number)
-                    rec.listed = key_logit(order_key(rec.listed + 0.0f) - 1u);
-                if (rec.count <= kChunkList)
-                    rec.listed = -INFINITY;
-            }
+            if (rec.count <= kChunkList)
+                rec.listed = -INFINITY;
+        } else {
+#pragma unroll
+            for (int k = kEach - 1; k >= 0; --k)
+                if (x[k] == rec.max)
+                    rec.first = c.token(k);
+            rec.first = __ockl_wfred_min_u32(rec.first);
         }
     }
     rec.max += 0.0f;
@@ -168,7 +182,7 @@ __global__ void __launch_bounds__(256, 8) scan_kernel(mako_cut_desc d, Scratch s
 }
 
 template <class E>
-__global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch sc)
+__global__ void __launch_bounds__(256, 4) look_kernel(mako_cut_desc d, Scratch sc)
 {
     __shared__ float weighed[4][kChunk];
     const uint32_t chunks = chunks_of(d.n_vocab), groups = (chunks + 3) / 4, items = sc.wide[0] * groups;
@@ -185,33 +199,34 @@ __global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch s
         if (max == kFltMax)
             c.no_infinity();
         ChunkRec rec = {0.0, 0.0f, 0.0f, 0u, 0u, 0u, 0.0f};
-        unsigned long long in[16];
-        const unsigned long long before = (1ull << lane()) - 1ull;
         // (what is weighed moves together first: where it is one logit in ten, nearly every 64 have one)
         float* const mine = weighed[wave()];
+        const uint64_t at = (uint64_t)row * sc.chunks_cap + chunk;
+        uint64_t* list = sc.looks + at * kLookList;
         uint32_t n = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < kEach; ++k) {
             const float x = c.x[k];
-            const unsigned long long up = __ballot(x >= high);
-            in[k] = __ballot(x >= low) & ~up;
-            rec.count += (uint32_t)__popcll(up);
-            rec.n_list += (uint32_t)__popcll(in[k]);
-            const unsigned long long side = from_above ? up : __ballot(x > -INFINITY) & ~(up | in[k]);
+            const bool up = x >= high, in = x >= low && !up, weigh = from_above ? up : x < low && x > -INFINITY;
+            const unsigned long long all = __ballot(in), side = __ballot(weigh);
+            rec.count += (uint32_t)__popcll(__ballot(up));
+            if (all) {
+                const uint32_t more = (uint32_t)__popcll(all);
+                if (rec.n_list + more <= kLookList)
+                    c.put(list, k, in, all, rec.n_list);
+                rec.n_list += more;
+            }
             if (side) {
-                if (side >> lane() & 1ull)
-                    mine[n + (uint32_t)__popcll(side & before)] = x;
+                if (weigh)
+                    mine[n + lanes_before(side)] = x;
                 n += (uint32_t)__popcll(side);
             }
         }
-        const uint64_t at = (uint64_t)row * sc.chunks_cap + chunk;
-        if (rec.n_list <= kChunkList)
-            c.list(in, sc.lists + at * kChunkList);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         double sum = 0.0;
         for (uint32_t i = (uint32_t)lane(); i < n; i += 64u)
-            sum += weight(mine[i], (double)max, scale);
+            sum += weight<true>(mine[i], (double)max, scale);
         __builtin_amdgcn_wave_barrier();
         rec.sum = __ockl_wfred_add_f64(sum);
         if (lane() == 0)

@@ -90,6 +90,8 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     if (e == hipSuccess)
         e = take(sc.lists, rows * sc.chunks_cap * mako::step::kChunkList);
     if (e == hipSuccess)
+        e = take(sc.looks, rows * sc.chunks_cap * mako::step::kLookList);
+    if (e == hipSuccess)
         e = take(sc.plans, rows);
     if (e == hipSuccess)
         e = take(sc.wide, rows + 1);
@@ -123,7 +125,7 @@ void mako_step_destroy(mako_step_ctx* ctx)
     {
         const OnDevice on(ctx->device);
         mako::step::Scratch& sc = ctx->sc;
-        void* ptrs[] = {sc.chunks, sc.lists, sc.plans, sc.wide, sc.parts, sc.stop, sc.released, sc.taken, sc.held, sc.free_state};
+        void* ptrs[] = {sc.chunks, sc.lists, sc.looks, sc.plans, sc.wide, sc.parts, sc.stop, sc.released, sc.taken, sc.held, sc.free_state};
         for (void* p : ptrs)
             if (p)
                 (void)hipFree(p);

@@ -51,23 +51,28 @@ struct F16 {
     }
 };
 
-// Logits i .. i + kVec - 1 of a row of n, as fp32; those at n and behind are NaN (no token).
+// Logits i .. i + kVec - 1 of a row, as fp32.
+template <class E>
+__device__ __forceinline__ void load_whole(const void* row, uint32_t i, float* x)
+{
+    using raw = typename E::raw;
+    const typename E::words w = *reinterpret_cast<const typename E::words*>(static_cast<const raw*>(row) + i);
+#pragma unroll
+    for (uint32_t k = 0; k < E::kVec; ++k)
+        x[k] = E::of(sizeof(raw) == 4 ? w[k % 4] : w[k / 2], (int)k);
+}
+// ... of a row of n; those at n and behind are NaN (no token).
 template <class E>
 __device__ __forceinline__ void load_vec(const void* row, uint32_t i, uint32_t n, float* x)
 {
-    using raw = typename E::raw;
-    const raw* p = static_cast<const raw*>(row) + i;
     if (i + E::kVec <= n) {
-        const typename E::words w = *reinterpret_cast<const typename E::words*>(p);
-#pragma unroll
-        for (uint32_t k = 0; k < E::kVec; ++k)
-            x[k] = E::of(sizeof(raw) == 4 ? w[k % 4] : w[k / 2], (int)k);
+        load_whole<E>(row, i, x);
     } else {
 #pragma unroll
         for (uint32_t k = 0; k < E::kVec; ++k) {
             x[k] = __uint_as_float(0x7fc00000u);
             if (i + k < n)
-                x[k] = E::of(p[k], 0);
+                x[k] = E::of(static_cast<const typename E::raw*>(row)[i + k], 0);
         }
     }
 }
@@ -102,22 +107,24 @@ __device__ __forceinline__ float key_logit(uint32_t k)
     return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
-// 2^t for t <= 0: 2^round(t) times a polynomial in the rest, of degree 10 and constant term 1, the one whose largest
-// relative error over [-1/2, 1/2] is least (2.1e-16, found by exchange).  2^0 is exactly 1.  0 below 2^-1074.
+// 2^t for t <= 0: 2^round(t) times a polynomial in the rest, of degree 9, the one whose largest relative error over
+// [-1/2, 1/2] is least (found by exchange) with its constant term made 1: 2.7e-14 (degree 10: 2e-16, and an operation more for
+// each logit).  2^0 is exactly 1.  0 below 2^-1074.  kFinite: t is neither NaN nor -infinity.
+template <bool kFinite = false>
 __device__ __forceinline__ double exp2_down(double t)
 {
-    t = fmax(t, -1100.0);
+    if (!kFinite)
+        t = fmax(t, -1100.0);
     const double n = rint(t), f = t - n;
-    double p = 7.0372784767444307e-09;
-    p = fma(p, f, 1.020853789089708e-07);
-    p = fma(p, f, 1.3215662838949978e-06);
-    p = fma(p, f, 1.5252658116637374e-05);
-    p = fma(p, f, 0.00015403529961119085);
-    p = fma(p, f, 0.0013333558228561327);
-    p = fma(p, f, 0.0096181291080346051);
-    p = fma(p, f, 0.055504108664458832);
-    p = fma(p, f, 0.24022650695908768);
-    p = fma(p, f, 0.69314718055994973);
+    double p = 1.0150344092361341e-07;
+    p = fma(p, f, 1.325940551832952e-06);
+    p = fma(p, f, 1.5252984798658376e-05);
+    p = fma(p, f, 0.0001540343494852222);
+    p = fma(p, f, 0.0013333557617675399);
+    p = fma(p, f, 0.0096181291920665896);
+    p = fma(p, f, 0.055504108668685152);
+    p = fma(p, f, 0.24022650695649655);
+    p = fma(p, f, 0.69314718055987101);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
 }
@@ -128,9 +135,10 @@ __device__ __forceinline__ double weight_scale(float temperature)
     return temperature > 0.0f ? fmax(kLog2e / (double)temperature, 1e-300) : 1e-300;
 }
 // (the difference first: it is exactly 0 for the largest logit, whose weight is exactly 1)
+template <bool kFinite = false>
 __device__ __forceinline__ double weight(float x, double max_logit, double scale)
 {
-    return exp2_down(((double)x - max_logit) * scale);
+    return exp2_down<kFinite>(((double)x - max_logit) * scale);
 }
 
 __device__ __forceinline__ int lane()

@@ -10,6 +10,9 @@ namespace step {
 // Largest top_k that is looked for in the chunks' lists.
 constexpr uint32_t kListTopK = 1024;
 
+// Rows of no more logits than this are held whole where they are cut, and have no lists.
+constexpr uint32_t kWholeRow = 6144;
+
 struct RowKind {
     bool greedy, cut; // cut: something may be cut off it, and the chunks' first tokens are wanted
     bool min_p, top_p;

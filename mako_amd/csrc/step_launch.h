@@ -9,9 +9,10 @@
 namespace mako {
 namespace step {
 
-// A row is read in chunks of 1024 logits, a wave each.
-constexpr uint32_t kChunk = 1024;
+// A row is read in chunks of 2048 logits, a wave each.
+constexpr uint32_t kChunk = 2048;
 constexpr uint32_t kChunkList = 64; // a chunk's first tokens that are written out, at most
+constexpr uint32_t kLookList = 256; // ... and those around the row's cut
 
 // (what the second pass over a row, around its cut, finds in a chunk takes the same place: `sum` of the tokens that are weighed,
 // `count` of those above, `n_list` in the list)
@@ -21,7 +22,7 @@ struct ChunkRec {
     float listed;    // all tokens of this logit and above are in the list; +inf: none
     uint32_t count;  // tokens
     uint32_t n_list;
-    uint32_t first;  // the first token of the largest logit
+    uint32_t first;  // the first token of the largest logit (rows without lists)
     float low;       // the smallest logit (rows with a min_p)
 };
 
@@ -37,7 +38,8 @@ struct RowPlan {
 
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
-    uint64_t* lists;      // [rows][chunks_cap][kChunkList]: (order key, token)
+    uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that
+    uint64_t* looks;      // [rows][chunks_cap][kLookList]
     uint32_t chunks_cap;  // of a row
     RowPlan* plans;       // [rows]
     uint32_t* wide;       // [rows + 1]: how many rows have a plan, and which
