@@ -27,11 +27,15 @@ typedef unsigned long long u64;
 struct RowLds {
     uint64_t list[kList];
     uint64_t small[kSmall];
+    uint64_t crowd[kCrowd];
     u64 small_units[kCrowd];
     u64 mass[kBins]; // weights in units of 2^-unit
     uint32_t count[kBins];
+    uint32_t ids[kBins];
     Share<kWaves> share;
     uint32_t counts[kWaves];
+    double squares[kWaves];
+    uint32_t first_bin[2], last_bin[2], n_before[2], n_upto[2];
     uint32_t n, at, before, id, first;
     u64 mass_before;
     double m;
@@ -183,16 +187,80 @@ __device__ void sort_list(uint64_t* list, uint32_t n)
         }
 }
 
+// How many of n equal tokens are before the cut, behind `count` tokens of `mass`; it is within them.
+__device__ __forceinline__ uint32_t rank_of_equals(const Want& want, uint32_t n, uint32_t count, double mass, double w)
+{
+    if (want.rank)
+        return want.rank - count;
+    const double r = ceil((want.mass - mass) / w);
+    return r >= (double)n ? n : (r < 1.0 ? 1u : (uint32_t)r);
+}
+
 // The cut in a list of n tokens that holds it, behind `count` tokens of `mass` that come before.
 template <class E>
 __device__ Cut cut_in_list(const Row<E>& row, const Want& want, uint64_t* list, uint32_t n, uint32_t count, double mass, RowLds& lds)
 {
+    // many equal logits (of 16 bits, most): the cut is behind so many of them, in the tokens' order
+    const uint32_t key = (uint32_t)(list[0] >> 32);
+    bool equal = n > 32u;
+    if (equal) {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+            equal = equal && (uint32_t)(list[i] >> 32) == key;
+        for (uint32_t i = threadIdx.x; i < kBins; i += kThreads)
+            lds.ids[i] = 0;
+        equal = all_min<kWaves>(equal, lds.share);
+    }
+    if (equal) {
+        const float v = key_logit(key);
+        const double w = row.weigh(v);
+        const uint32_t rank = rank_of_equals(want, n, count, mass, w);
+        const uint32_t shift = row.n > kBins ? 22u - (uint32_t)__builtin_clz(row.n - 1u) : 0u; // (tokens to bins)
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+            atomicAdd(&lds.ids[(uint32_t)list[i] >> shift], 1u);
+        if (threadIdx.x == 0)
+            lds.n = 0;
+        __syncthreads();
+        const uint32_t a = 2 * threadIdx.x, c[2] = {lds.ids[a], lds.ids[a + 1]};
+        u64 all;
+        uint32_t before = (uint32_t)sum_before<kWaves>((u64)(c[0] + c[1]), all, lds.share);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (before < rank && rank <= before + c[k]) {
+                lds.at = a + (uint32_t)k;
+                lds.before = before;
+            }
+            before += c[k];
+        }
+        __syncthreads();
+        const uint32_t bin = lds.at, in_bin = rank - lds.before;
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+            if ((uint32_t)list[i] >> shift == bin) {
+                const uint32_t at = atomicAdd(&lds.n, 1u);
+                lds.ids[at] = (uint32_t)list[i]; // (a bin has 1024 tokens at most, of 2^20)
+            }
+        __syncthreads();
+        const uint32_t crowd = lds.n;
+        for (uint32_t i = threadIdx.x; i < crowd; i += kThreads) {
+            uint32_t place = 0;
+            for (uint32_t j = 0; j < crowd; ++j)
+                place += lds.ids[j] <= lds.ids[i];
+            if (place == in_bin)
+                lds.id = lds.ids[i];
+        }
+        __syncthreads();
+        const Cut cut = {count + rank, mass + (double)rank * w, v, lds.id};
+        __syncthreads();
+        return cut;
+    }
     if (n <= kCrowd) {
         // every token's place, and what those up to it weigh, by a look at all the others: no order needs to be made
+        // (eight at a time, in an array that is filled up with what is behind all)
         uint64_t mine = ~0ull;
-        if (threadIdx.x < n) {
-            mine = list[threadIdx.x];
-            lds.small_units[threadIdx.x] = row.units(row.weigh(key_logit((uint32_t)(mine >> 32))));
+        if (threadIdx.x < kCrowd) {
+            if (threadIdx.x < n)
+                mine = list[threadIdx.x];
+            lds.crowd[threadIdx.x] = mine;
+            lds.small_units[threadIdx.x] = threadIdx.x < n ? row.units(row.weigh(key_logit((uint32_t)(mine >> 32)))) : 0ull;
         }
         if (threadIdx.x == 0)
             lds.at = kNoToken;
@@ -200,11 +268,13 @@ __device__ Cut cut_in_list(const Row<E>& row, const Want& want, uint64_t* list, 
         uint32_t place = 0;
         u64 upto = 0;
         if (threadIdx.x < ((n + 63u) & ~63u)) {
-            for (uint32_t i = 0; i < n; ++i) {
-                const bool before = list[i] <= mine;
-                place += before;
-                upto += before ? lds.small_units[i] : 0ull;
-            }
+            for (uint32_t i = 0; i < n; i += 8u)
+#pragma unroll
+                for (uint32_t k = 0; k < 8u; ++k) {
+                    const bool before = lds.crowd[i + k] <= mine && i + k < n;
+                    place += before;
+                    upto += before ? lds.small_units[i + k] : 0ull;
+                }
             if (threadIdx.x < n && (place == n || want.reached(count + place, mass + row.mass(upto))))
                 atomicMin(&lds.at, place);
         }
@@ -316,11 +386,7 @@ __device__ Cut cut_by_division(Row<E>& row, const Want& want, double total, uint
         // nothing but equal logits: the cut is behind so many of them, in the tokens' order
         const float v = key_logit(prefix);
         const double w = row.weigh(v);
-        uint32_t rank = want.rank - before;
-        if (!want.rank) {
-            const double r = ceil((want.mass - row.mass(mass_before)) / w);
-            rank = r >= (double)bin.n ? bin.n : (r < 1.0 ? 1u : (uint32_t)r);
-        }
+        const uint32_t rank = rank_of_equals(want, bin.n, before, row.mass(mass_before), w);
         uint32_t seen = 0;
         constexpr uint32_t kStep = kThreads * E::kVec;
         for (uint32_t base = 0; base < row.n && seen < rank; base += kStep) {
@@ -384,69 +450,97 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
                     atomicAdd(&lds.count[bins.of(v[a][k])], 1u);
     }
     __syncthreads();
+    // running sums of the bins, by rank of their tokens alone, by mass of what these weigh and of its squares too
     const uint32_t a = 2 * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
-    u64 all;
-    uint32_t upto = (uint32_t)sum_before<kWaves>((u64)(c[0] + c[1]), all, lds.share);
-    const uint32_t samples = (uint32_t)all;
+    double w[2] = {}, sum = 0.0, squares = 0.0;
+    if (!plan.rank) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            w[k] = row.weigh(bins.top - (float)(((double)(a + k) + 0.5) / (double)bins.scale));
+            sum += w[k] * c[k];
+            squares += w[k] * w[k] * c[k];
+        }
+        sum = __ockl_wfscan_add_f64(sum, true);
+        squares = __ockl_wfscan_add_f64(squares, true);
+    }
+    uint32_t upto = __ockl_wfscan_add_u32(c[0] + c[1], true);
+    if (lane() == 63) {
+        lds.counts[wave()] = upto;
+        lds.share.d[wave()] = sum;
+        lds.squares[wave()] = squares;
+    }
+    if (threadIdx.x == 0)
+        lds.first_bin[0] = lds.last_bin[0] = lds.first_bin[1] = lds.last_bin[1] = 0;
+    __syncthreads();
+    uint32_t samples = 0, n_all = 0;
+    double sums = 0.0, sum_all = 0.0, squares_before = 0.0, squares_all = 0.0;
+    for (int v = 0; v < kWaves; ++v) {
+        if (v == wave()) {
+            n_all = samples;
+            sum_all = sums;
+            squares_before = squares_all;
+        }
+        samples += lds.counts[v];
+        sums += lds.share.d[v];
+        squares_all += lds.squares[v];
+    }
     if (samples == 0)
         return;
-    const double each = (double)plan.tokens / (double)samples;
-    // by rank: tokens of the bins up to this one; by mass: what the tokens behind them weigh.  With the deviation of either.
-    double far[2], dev[2]; // (far grows from bin to bin, and is 0 where the cut is)
-    if (plan.rank) {
-        uint32_t n = upto;
+    upto += n_all;
+    sum += sum_all;
+    squares += squares_before;
+    // how far behind the cut a bin's end is (it grows from bin to bin), and the deviation of that: by rank in tokens up to there,
+    // by mass in what the tokens behind it weigh.  (A sample that holds one of the row's few heavy tokens has both far off in the
+    // bins up to it.)  The cut is behind the last bin whose end is surely before it, and in the one behind the last whose end may be
+    // before it, or sooner.
+    const double each = (double)plan.tokens / (double)samples, behind_goal = plan.total - plan.mass;
+    double behind = sums - sum, var = squares_all - squares;
+    uint32_t n = upto, first[2] = {}, last[2] = {};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            n += c[k];
-            far[k] = (double)n * each - (double)plan.rank;
-            dev[k] = each * sqrt((double)n + 1.0);
+    for (int k = 1; k >= 0; --k) {
+        const double far = plan.rank ? (double)n * each - (double)plan.rank : behind_goal - behind * each;
+        const double dev = each * sqrt(plan.rank ? (double)n + 1.0 : fmax(var, 0.0));
+#pragma unroll
+        for (int tries = 0; tries < 2; ++tries) {
+            const double z = tries ? 2.0 : 3.0;
+            if (far < -z * dev)
+                first[tries] = max(first[tries], a + (uint32_t)k + 1u);
+            if (far < z * dev)
+                last[tries] = max(last[tries], a + (uint32_t)k + 1u);
         }
-    } else {
-        double w[2], sum, sums;
+        n -= c[k];
+        behind += w[k] * c[k];
+        var += w[k] * w[k] * c[k];
+    }
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            w[k] = each * row.weigh(bins.top - (float)(((double)(a + k) + 0.5) / (double)bins.scale));
-        sum = sum_before<kWaves>(w[0] * c[0] + w[1] * c[1], sums, lds.share);
-        double behind = sums - sum;
-        sum = sum_before<kWaves>(w[0] * w[0] * c[0] + w[1] * w[1] * c[1], sums, lds.share);
-        double var = sums - sum;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            behind -= w[k] * c[k];
-            var -= w[k] * w[k] * c[k];
-            far[k] = plan.total - plan.mass - behind;
-            dev[k] = sqrt(fmax(var, 0.0));
+    for (int tries = 0; tries < 2; ++tries) {
+        first[tries] = __ockl_wfred_max_u32(first[tries]);
+        last[tries] = __ockl_wfred_max_u32(last[tries]);
+        if (lane() == 0) {
+            atomicMax(&lds.first_bin[tries], first[tries]);
+            atomicMax(&lds.last_bin[tries], last[tries]);
         }
     }
-    // (a sample that holds one of the row's few heavy tokens has both far off in the bins up to it: the cut is behind the last bin
-    // that is surely before it, and in or before the first one behind that by which it surely is)
+    __syncthreads();
+#pragma unroll
     for (int tries = 0; tries < 2; ++tries) {
-        const double z = tries ? 2.0 : 3.0;
-        uint32_t first = 0, last = kNoToken, n = upto;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (far[k] < -z * dev[k])
-                first = a + (uint32_t)k + 1u;
-        const uint32_t first_bin = ~all_min<kWaves>(~first, lds.share);
-#pragma unroll
-        for (int k = 1; k >= 0; --k)
-            if (a + (uint32_t)k >= first_bin && far[k] >= z * dev[k])
-                last = a + (uint32_t)k;
-        const uint32_t last_bin = all_min<kWaves>(last, lds.share);
+        n = upto - c[0] - c[1];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            if (a + (uint32_t)k == first_bin)
-                lds.before = n;
+            if (a + (uint32_t)k == lds.first_bin[tries])
+                lds.n_before[tries] = n;
             n += c[k];
-            if (a + (uint32_t)k == last_bin)
-                lds.n = n;
+            if (a + (uint32_t)k == lds.last_bin[tries])
+                lds.n_upto[tries] = n;
         }
-        __syncthreads();
-        const uint32_t n_before = lds.before, n_bins = lds.n - n_before;
-        __syncthreads();
+    }
+    __syncthreads();
+    for (int tries = 0; tries < 2; ++tries) {
+        const uint32_t first_bin = lds.first_bin[tries], last_bin = lds.last_bin[tries];
         if (last_bin >= kBins - 1u) // (the last bin has no lower end)
             return;
+        const uint32_t n_before = lds.n_before[tries], n_bins = lds.n_upto[tries] - n_before;
         if ((double)n_bins * each > 0.9 * kList)
             continue;
         plan.high = first_bin ? bins.top - (float)((double)first_bin / (double)bins.scale) : INFINITY;
@@ -546,10 +640,7 @@ struct Lists {
                 lds.list[place] = (uint64_t)order_key(x + 0.0f) << 32 | (uint32_t)e;
         };
         u64 in[kAhead];
-        uint32_t n = 0, longest = 0;
-#pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h)
-            longest = ::max(longest, c.rec[h].n_list);
+        uint32_t n = 0;
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
             const uint32_t of_chunk = (uint32_t)__shfl((int)c.rec[a * kOfAll / 64u].n_list, (int)(chunk(a) & 63u));
@@ -566,8 +657,7 @@ struct Lists {
             at += (uint32_t)__popcll(in[a]);
         }
         // longer lists, and the chunks beyond
-        auto rest = [&](uint32_t i, uint32_t slot) {
-            const uint32_t of_chunk = recs[i].n_list;
+        auto rest = [&](uint32_t i, uint32_t slot, uint32_t of_chunk) {
             for (; slot < of_chunk; slot += 64u) {
                 const uint64_t e = slot + (uint32_t)lane() < of_chunk ? lists[i * kRoom + slot + (uint32_t)lane()] : 0ull;
                 const bool in_list = slot + (uint32_t)lane() < of_chunk && __uint_as_float((uint32_t)(e >> 32)) >= from;
@@ -579,11 +669,15 @@ struct Lists {
                 put(e, in_list, to + (uint32_t)__popcll(more & before));
             }
         };
-        if (__ballot(longest > kSlots))
-            for (uint32_t i = (uint32_t)wave(); i < min(chunks, kAhead * kOfAll); i += kWaves)
-                rest(i, kSlots);
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h)
+            for (u64 left = __ballot(c.rec[h].n_list > kSlots); left; left &= left - 1u) {
+                const uint32_t i = (uint32_t)__builtin_ctzll(left);
+                if (i % kWaves == (uint32_t)wave() && h * 64u + i < kAhead * kOfAll)
+                    rest(h * 64u + i, kSlots, (uint32_t)__builtin_amdgcn_readlane((int)c.rec[h].n_list, (int)i));
+            }
         for (uint32_t i = kAhead * kOfAll + (uint32_t)wave(); i < chunks; i += kWaves)
-            rest(i, 0u);
+            rest(i, 0u, recs[i].n_list);
         __syncthreads();
         const uint32_t all = lds.n;
         __syncthreads();
@@ -615,13 +709,14 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     const uint64_t* lists = sc.lists + (uint64_t)r * sc.chunks_cap * kChunkList;
     Chunks c;
     c.load(recs, chunks);
-    const mako_sampling_params p = d.params[r / d.rows_per_params];
-    const RowKind kind(p);
+    // (before the row's parameters are known: a row that is not cut has no lists, and what is there is not looked at)
     FirstLists listed;
     const bool whole = d.n_vocab <= kWholeRow;
+    if (!whole)
+        listed.load(lists, chunks);
+    const mako_sampling_params p = d.params[r / d.rows_per_params];
+    const RowKind kind(p);
     if (kind.cut) {
-        if (!whole)
-            listed.load(lists, chunks);
         clear_bins(lds);
         if (threadIdx.x == 0) {
             lds.n = 0;
@@ -688,8 +783,18 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         }
     }
     if (!all_weighty && row.weigh(c.low) < (double)p.min_p) {
+        // the least logit that weighs enough, between the smallest, which does not, and the largest, by halving their order keys
+        uint32_t enough = order_key(row.max), less = order_key(c.low);
+        while (less - enough > 1u) {
+            const uint32_t middle = enough + (less - enough) / 2u;
+            if (row.weigh(key_logit(middle)) >= (double)p.min_p)
+                enough = middle;
+            else
+                less = middle;
+        }
+        const float least = key_logit(enough);
         uint32_t above = 0;
-        row.each([&](uint32_t, float v) { above += row.weigh(v) >= (double)p.min_p; });
+        row.each([&](uint32_t, float v) { above += v >= least; });
         rank = min(rank, max(all_sum<kWaves>(above, lds.share), 1u));
     }
     Cut cut = {c.count, c.total, 0.0f, 0};
@@ -719,15 +824,18 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     // the cut lies further down
     plan.total = c.total;
     plan.tokens = c.count;
-    plan.look = 0;
+    plan.low = plan.high = 0.0f;
+    plan.from_above = plan.look = 0;
     // (where it is to be expected: within four times what lies between the largest logit and the one of the mean weight, or, where
     // that is not known, twice what the lists reach down)
     const double range = kind.sums ? 4.0 * log((double)c.count / c.total) * kLog2e / row.scale : 2.0 * ((double)row.max - (double)c.listed);
     if ((kind.sums || plan.rank) && range > 0.0 && range < 1e30)
         guess(row, range, plan, lds);
     if (threadIdx.x == 0) {
-        sc.plans[r] = plan;
-        sc.wide[1 + atomicAdd(&sc.wide[0], 1u)] = r;
+        plan.row = r;
+        plan.max = row.max;
+        plan.scale = row.scale;
+        sc.plans[atomicAdd(sc.wide, 1u)] = plan;
     }
 }
 
@@ -736,16 +844,16 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
 {
     extern __shared__ unsigned char dyn[];
     RowLds& lds = *reinterpret_cast<RowLds*>(dyn);
-    const uint32_t rows = sc.wide[0], chunks = chunks_of(d.n_vocab);
+    const uint32_t rows = *sc.wide, chunks = chunks_of(d.n_vocab);
     for (uint32_t i = blockIdx.x; i < rows; i += gridDim.x) {
-        const uint32_t r = sc.wide[1 + i];
-        const RowPlan plan = sc.plans[r];
+        const RowPlan plan = sc.plans[i];
+        const uint32_t r = plan.row;
         const ChunkRec* recs = sc.chunks + (uint64_t)r * sc.chunks_cap;
         const uint64_t* lists = sc.looks + (uint64_t)r * sc.chunks_cap * kLookList;
         const mako_sampling_params p = d.params[r / d.rows_per_params];
         const RowKind kind(p);
         mako_row_cut& out = d.out_cuts[r];
-        Row<E> row(d, r, out.max_logit, kind.scale);
+        Row<E> row(d, r, plan.max, plan.scale);
         Want want = {plan.rank, plan.mass};
         Cut cut = {0, 0.0, 0.0f, 0};
         double total = plan.total;

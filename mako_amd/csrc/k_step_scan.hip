@@ -25,26 +25,24 @@ __device__ __forceinline__ float nth_largest(float v, uint32_t n)
     return key_logit(~found);
 }
 
-constexpr int kEach = kChunk / 64; // logits of a lane
-
 __device__ __forceinline__ uint32_t lanes_before(unsigned long long lanes)
 {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
 }
 
-// A chunk's logits; -inf: no token.
-template <class E>
-struct Chunk {
+// 64 kEach logits of a row, from token `begin` on; -inf: no token.
+template <class E, int kEach>
+struct Logits {
     uint32_t begin;
     float x[kEach];
 
     // (the k-th logit's token)
     __device__ __forceinline__ uint32_t token(int k) const { return begin + ((uint32_t)k / E::kVec * 64u + (uint32_t)lane()) * E::kVec + (uint32_t)k % E::kVec; }
 
-    __device__ __forceinline__ Chunk(const mako_cut_desc& d, uint32_t row, uint32_t chunk) : begin(chunk * kChunk)
+    __device__ __forceinline__ Logits(const mako_cut_desc& d, uint32_t row, uint32_t from) : begin(from)
     {
         const void* x_row = static_cast<const typename E::raw*>(d.logits) + (int64_t)row * d.logits_stride;
-        if (begin + kChunk <= d.n_vocab) {
+        if (begin + 64u * kEach <= d.n_vocab) {
 #pragma unroll
             for (int k = 0; k < kEach; k += (int)E::kVec)
                 load_whole<E>(x_row, token(k), x + k);
@@ -88,10 +86,11 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
 {
     const uint32_t row = blockIdx.y, chunk = blockIdx.x * 4u + (uint32_t)wave(), chunks = chunks_of(d.n_vocab);
     if (row == 0 && chunk == 0 && lane() == 0)
-        sc.wide[0] = 0;
+        *sc.wide = 0;
     if (chunk >= chunks)
         return;
-    Chunk<E> c(d, row, chunk);
+    constexpr int kEach = kChunk / 64;
+    Logits<E, kEach> c(d, row, chunk * kChunk);
     const float(&x)[kEach] = c.x;
     const RowKind kind(d.params[row / d.rows_per_params]);
     float mine = x[0], low = x[0];
@@ -182,52 +181,56 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
 }
 
 template <class E>
-__global__ void __launch_bounds__(256, 4) look_kernel(mako_cut_desc d, Scratch sc)
+__global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch sc)
 {
-    __shared__ float weighed[4][kChunk];
-    const uint32_t chunks = chunks_of(d.n_vocab), groups = (chunks + 3) / 4, items = sc.wide[0] * groups;
+    constexpr int kEach = 16; // (a chunk in two halves: the more waves, the less they wait for)
+    __shared__ float weighed[4][64 * kEach];
+    const uint32_t chunks = chunks_of(d.n_vocab), groups = (chunks + 3) / 4, items = *sc.wide * groups;
     for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t row = sc.wide[1 + item / groups], chunk = item % groups * 4u + (uint32_t)wave();
-        const RowPlan& plan = sc.plans[row];
+        const RowPlan& plan = sc.plans[item / groups];
+        const uint32_t row = plan.row, chunk = item % groups * 4u + (uint32_t)wave();
+        const float low = plan.low, high = plan.high, max = plan.max;
+        const double scale = plan.scale;
+        const bool from_above = plan.from_above;
         if (!plan.look || chunk >= chunks)
             continue;
-        const float low = plan.low, high = plan.high;
-        const bool from_above = plan.from_above;
-        const float max = d.out_cuts[row].max_logit;
-        const double scale = weight_scale(d.out_cuts[row].temperature);
-        Chunk<E> c(d, row, chunk);
-        if (max == kFltMax)
-            c.no_infinity();
         ChunkRec rec = {0.0, 0.0f, 0.0f, 0u, 0u, 0u, 0.0f};
         // (what is weighed moves together first: where it is one logit in ten, nearly every 64 have one)
         float* const mine = weighed[wave()];
         const uint64_t at = (uint64_t)row * sc.chunks_cap + chunk;
         uint64_t* list = sc.looks + at * kLookList;
-        uint32_t n = 0;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            const float x = c.x[k];
-            const bool up = x >= high, in = x >= low && !up, weigh = from_above ? up : x < low && x > -INFINITY;
-            const unsigned long long all = __ballot(in), side = __ballot(weigh);
-            rec.count += (uint32_t)__popcll(__ballot(up));
-            if (all) {
-                const uint32_t more = (uint32_t)__popcll(all);
-                if (rec.n_list + more <= kLookList)
-                    c.put(list, k, in, all, rec.n_list);
-                rec.n_list += more;
-            }
-            if (side) {
-                if (weigh)
-                    mine[n + lanes_before(side)] = x;
-                n += (uint32_t)__popcll(side);
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
         double sum = 0.0;
-        for (uint32_t i = (uint32_t)lane(); i < n; i += 64u)
-            sum += weight<true>(mine[i], (double)max, scale);
-        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (uint32_t begin = chunk * kChunk; begin < min((chunk + 1u) * kChunk, d.n_vocab); begin += 64u * kEach) {
+            Logits<E, kEach> c(d, row, begin);
+            if (max == kFltMax)
+                c.no_infinity();
+            uint32_t n = 0;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const float x = c.x[k];
+                const bool up = x >= high, in = x >= low && !up, weigh = from_above ? up : x < low && x > -INFINITY;
+                const unsigned long long all = __ballot(in), side = __ballot(weigh);
+                rec.count += (uint32_t)__popcll(__ballot(up));
+                if (all) {
+                    const uint32_t more = (uint32_t)__popcll(all);
+                    if (rec.n_list + more <= kLookList)
+                        c.put(list, k, in, all, rec.n_list);
+                    rec.n_list += more;
+                }
+                if (side) {
+                    if (weigh)
+                        mine[n + lanes_before(side)] = x;
+                    n += (uint32_t)__popcll(side);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (uint32_t i = (uint32_t)lane(); i < n; i += 64u)
+                sum += weight<true>(mine[i], (double)max, scale);
+            __builtin_amdgcn_wave_barrier();
+        }
         rec.sum = __ockl_wfred_add_f64(sum);
         if (lane() == 0)
             sc.chunks[at] = rec;

@@ -94,7 +94,7 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     if (e == hipSuccess)
         e = take(sc.plans, rows);
     if (e == hipSuccess)
-        e = take(sc.wide, rows + 1);
+        e = take(sc.wide, 1);
     if (e == hipSuccess)
         e = take(sc.parts, rows * sc.parts_cap);
     if (e == hipSuccess)

@@ -30,7 +30,9 @@ struct ChunkRec {
 struct RowPlan {
     double mass, total; // the cut is behind the first tokens that weigh `mass`, of all that weigh `total` (0: not known),
     uint32_t rank;      // or, if not 0, behind the first `rank`
-    uint32_t tokens;    // of the row
+    uint32_t row, tokens; // which row, and how many tokens it has
+    float max;          // its largest logit
+    double scale;       // log2(e) / T
     float low, high;    // the tokens from `low` up to `high` are listed,
     uint32_t from_above; // those above are weighed, or those below
     uint32_t look;       // 0: there is no guess where it lies
@@ -41,8 +43,8 @@ struct Scratch {
     uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that
     uint64_t* looks;      // [rows][chunks_cap][kLookList]
     uint32_t chunks_cap;  // of a row
-    RowPlan* plans;       // [rows]
-    uint32_t* wide;       // [rows + 1]: how many rows have a plan, and which
+    RowPlan* plans;       // [rows]: of those that have one, in no order
+    uint32_t* wide;       // [1]: how many do
     double* parts;        // [rows][parts_cap]: what is left to draw from in each part of the row where a request stops
     uint32_t parts_cap;
     uint32_t* stop;       // [rows] drafts a request accepts
