@@ -914,6 +914,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
     }
 }
 
+constexpr uint32_t kProbs = 4096; // logits of a workgroup
 template <class E>
 __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
 {
@@ -924,16 +925,29 @@ __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
     float* out = d.out_probs + (int64_t)r * d.probs_stride;
     const double scale = weight_scale(c.temperature), md = (double)c.max_logit, share = c.total > 0.0 ? 1.0 / c.total : 0.0;
     for (uint32_t j = 0; j < 16u / E::kVec; ++j) {
-        const uint32_t i = blockIdx.x * kPart + (j * 256u + threadIdx.x) * E::kVec;
+        const uint32_t i = blockIdx.x * kProbs + (j * 256u + threadIdx.x) * E::kVec;
         if (i >= d.n_vocab)
             break;
-        float x[E::kVec];
+        float x[E::kVec], p[E::kVec];
         load_tokens<E>(x_row, mask, i, d.n_vocab, x);
 #pragma unroll
         for (uint32_t k = 0; k < E::kVec; ++k) {
             const bool kept = x[k] > c.cut_logit || (x[k] == c.cut_logit && (int32_t)(i + k) <= c.cut_token);
-            if (i + k < d.n_vocab)
-                out[i + k] = kept ? (float)(weight(x[k], md, scale) * share) : 0.0f;
+            p[k] = 0.0f;
+            if (__ballot(kept))
+                p[k] = kept ? (float)(weight(x[k], md, scale) * share) : 0.0f;
+        }
+        if (i + E::kVec <= d.n_vocab) {
+#pragma unroll
+            for (uint32_t k = 0; k < E::kVec; k += 4u) {
+                const words_at_4 w = {__float_as_uint(p[k]), __float_as_uint(p[k + 1]), __float_as_uint(p[k + 2]), __float_as_uint(p[k + 3])};
+                *reinterpret_cast<words_at_4*>(out + i + k) = w;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < E::kVec; ++k)
+                if (i + k < d.n_vocab)
+                    out[i + k] = p[k];
         }
     }
 }
@@ -950,7 +964,7 @@ void cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 template <class E>
 void probs(hipStream_t st, const mako_cut_desc& d)
 {
-    hipLaunchKernelGGL(probs_kernel<E>, dim3((d.n_vocab + kPart - 1) / kPart, d.n_rows), dim3(256), 0, st, d);
+    hipLaunchKernelGGL(probs_kernel<E>, dim3((d.n_vocab + kProbs - 1) / kProbs, d.n_rows), dim3(256), 0, st, d);
 }
 
 } // namespace

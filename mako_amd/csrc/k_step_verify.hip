@@ -1,8 +1,8 @@
 // Verification of drafted tokens (mako_step_verify_drafts).
 //
-//   left_kernel  a workgroup for every part of 4096 tokens of every request: where the request stops accepting, and what
-//                the slice has left there to draw from
-//   draw_kernel  a workgroup for every request: the slice that the uniform falls into, and the token in it
+//   left_kernel  a workgroup for every part of 1024 tokens of every request, or for several: where the request stops accepting,
+//                which each of them finds out for itself, and what its parts have left there to draw from
+//   draw_kernel  a workgroup for every request: the part that the uniform falls into, and the token in it
 #include "step_common.h"
 #include "step_launch.h"
 
@@ -11,7 +11,8 @@ namespace step {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr uint32_t kRun = 8, kRuns = kPart / kThreads / kRun; // a thread has runs of 8 tokens: of either row, whatever its type
+constexpr uint32_t kMostParts = 32; // of a workgroup
+static_assert(kPart == 4 * kThreads, "four tokens to a thread");
 
 // A row of weights: logits under their cut, or probabilities.
 template <class E>
@@ -19,52 +20,62 @@ struct Row {
     const typename E::raw* x;
     const uint32_t* mask;
     uint32_t n;
-    bool probs;
+    bool probs, few;
     float cut;
     int32_t cut_token;
     double max, scale, share;
 
-    __device__ __forceinline__ Row(const void* base, int64_t stride, const uint32_t* masks, int64_t mask_stride, const mako_row_cut* cuts, uint32_t n_vocab, uint64_t row)
+    __device__ __forceinline__ Row(const void* base, int64_t stride, const uint32_t* masks, int64_t mask_stride, bool cuts, const StopRow& c, uint32_t n_vocab, uint64_t row)
         : x(static_cast<const typename E::raw*>(base) + (int64_t)row * stride), mask(cuts && masks ? masks + (int64_t)row * mask_stride : nullptr), n(n_vocab),
-          probs(!cuts), cut(0.0f), cut_token(-1), max(0.0), scale(0.0), share(0.0)
+          probs(!cuts), few(c.few), cut(c.cut), cut_token(c.cut_token), max(c.max), scale(c.scale), share(c.share)
     {
-        if (cuts) {
-            const mako_row_cut c = cuts[row];
-            cut = c.cut_logit;
-            cut_token = c.cut_token;
-            max = (double)c.max_logit;
-            scale = weight_scale(c.temperature);
-            share = c.total > 0.0 ? 1.0 / c.total : 0.0;
-        }
     }
-    __device__ __forceinline__ double prob(uint32_t i, float v) const // (v: as token_logit() gives it, or a probability)
+    // Whether a logit as it is in memory can be one of a kept token; probabilities: whether it is one.
+    __device__ __forceinline__ bool may_keep(float v) const { return probs ? v > 0.0f : v >= cut; }
+    // (v: as token_logit() gives it, or a probability)
+    __device__ __forceinline__ bool kept(uint32_t i, float v) const
     {
-        if (probs)
-            return v > 0.0f && v <= kFltMax ? (double)v : 0.0;
-        const bool kept = v > cut || (v == cut && (int32_t)i <= cut_token);
-        return kept ? weight(v, max, scale) * share : 0.0;
+        return probs ? v > 0.0f && v <= kFltMax : v > cut || (v == cut && (int32_t)i <= cut_token);
     }
-    __device__ __forceinline__ double one(uint32_t i) const
+    __device__ __forceinline__ double one(uint32_t i, float v, uint32_t bits) const
     {
-        if (i >= n)
+        if (!probs)
+            v = token_logit(v, bits >> (i & 31u) & 1u);
+        if (i >= n || !kept(i, v))
             return 0.0;
-        const float v = E::of(x[i], 0);
-        return prob(i, probs ? v : token_logit(v, !mask || (mask[i >> 5] >> (i & 31u) & 1u)));
+        return probs ? (double)v : weight(v, max, scale) * share;
     }
-    // kRun probabilities from token i on; 0 behind the row's end
-    __device__ __forceinline__ void run(uint32_t i, double* p) const
+    // four logits or probabilities from token i on, as they are in memory; whole: none is behind the row's end
+    __device__ __forceinline__ void load(uint32_t i, bool whole, float* v) const
     {
-        float v[kRun];
+        if (whole)
+            load_whole_four<E>(x, i, v);
+        else
+            load_four<E>(x, i, n, v);
+    }
+    // and the probabilities that these are
+    __device__ __forceinline__ void four(uint32_t i, const float* v, double* out) const
+    {
+        if (probs) {
 #pragma unroll
-        for (uint32_t h = 0; h < kRun; h += E::kVec) {
-            if (probs)
-                load_vec<E>(x, i + h, n, v + h);
-            else
-                load_tokens<E>(x, mask, i + h, n, v + h);
+            for (uint32_t k = 0; k < 4u; ++k)
+                out[k] = kept(i + k, v[k]) ? (double)v[k] : 0.0;
+            return;
         }
+        uint32_t bits = 0xffffffffu;
+        if (mask) // (the four bits lie in one word)
+            bits = i < n ? mask[i >> 5] >> (i & 31u) : 0u;
+        float x4[4];
+        double t[4];
 #pragma unroll
-        for (uint32_t k = 0; k < kRun; ++k)
-            p[k] = prob(i + k, v[k]);
+        for (uint32_t k = 0; k < 4u; ++k) {
+            x4[k] = token_logit(v[k], (bits >> k) & 1u);
+            t[k] = ((double)x4[k] - max) * scale;
+        }
+        exp2_down<4>(t, out);
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k)
+            out[k] = kept(i + k, x4[k]) ? out[k] * share : 0.0;
     }
 };
 
@@ -76,103 +87,214 @@ struct Left {
     bool minus_q;
     uint32_t without; // kNoToken: none
 
-    __device__ __forceinline__ void run(uint32_t i, double* r) const
-    {
-        p.run(i, r);
-        if (minus_q) {
-            double s[kRun];
-            q.run(i, s);
-#pragma unroll
-            for (uint32_t k = 0; k < kRun; ++k)
-                r[k] = fmax(r[k] - s[k], 0.0);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kRun; ++k)
-            if (i + k == without)
-                r[k] = 0.0;
-    }
     __device__ __forceinline__ void give_up()
     {
         minus_q = false;
         without = kNoToken;
     }
-    // (16 tokens of a slice of 4096 to a thread; the sum of the thread's own)
-    __device__ __forceinline__ double slice(uint32_t s, double* r) const
+    // p's tokens of a part, four to a thread, and q's
+    __device__ __forceinline__ void load(uint32_t at, float* v, float* w) const
     {
-        double sum = 0.0;
+        const bool whole = (at + 1u) * kPart <= p.n;
+        p.load(at * kPart + threadIdx.x * 4u, whole, v);
+        if (minus_q)
+            q.load(at * kPart + threadIdx.x * 4u, whole, w);
+    }
+    // and what they have left
+    __device__ __forceinline__ void four(uint32_t at, const float* v, const float* w, double* r) const
+    {
+        const uint32_t i = at * kPart + threadIdx.x * 4u;
+        bool any = false;
 #pragma unroll
-        for (uint32_t j = 0; j < kRuns; ++j)
-            run(s * kPart + (j * kThreads + threadIdx.x) * kRun, r + j * kRun);
+        for (uint32_t k = 0; k < 4u; ++k) {
+            any = any || p.may_keep(v[k]);
+            r[k] = 0.0;
+        }
+        if (!__ballot(any))
+            return;
+        p.four(i, v, r);
+        if (minus_q) {
+            double s[4];
+            q.four(i, w, s);
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            sum += r[k];
-        return sum;
+            for (uint32_t k = 0; k < 4u; ++k)
+                r[k] = fmax(r[k] - s[k], 0.0);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k)
+            if (i + k == without)
+                r[k] = 0.0;
+    }
+    __device__ __forceinline__ void part(uint32_t at, double* r) const
+    {
+        float v[4], w[4];
+        load(at, v, w);
+        four(at, v, w, r);
     }
 };
 
-__device__ __forceinline__ uint32_t drafts_of(const mako_verify_desc& d, uint32_t b, bool& there)
-{
-    const int32_t n = d.n_drafts ? d.n_drafts[b] : (int32_t)d.max_drafts;
-    there = n >= 0;
-    return there ? min((uint32_t)n, d.max_drafts) : 0u;
-}
-
 template <class E>
-__device__ __forceinline__ Row<E> target_row(const mako_verify_desc& d, uint64_t row)
+__device__ __forceinline__ Row<E> target_row(const mako_verify_desc& d, const StopRow& c, uint64_t row)
 {
-    return Row<E>(d.target, d.target_stride, d.target_mask, d.target_mask_stride, d.target_cuts, d.n_vocab, row);
+    return Row<E>(d.target, d.target_stride, d.target_mask, d.target_mask_stride, d.target_cuts != nullptr, c, d.n_vocab, row);
 }
 template <class E>
-__device__ __forceinline__ Row<E> draft_row(const mako_verify_desc& d, uint64_t row)
+__device__ __forceinline__ Row<E> draft_row(const mako_verify_desc& d, const StopRow& c, uint64_t row)
 {
-    return Row<E>(d.draft, d.draft_stride, d.draft_mask, d.draft_mask_stride, d.draft_cuts, d.n_vocab, row);
+    return Row<E>(d.draft, d.draft_stride, d.draft_mask, d.draft_mask_stride, d.draft_cuts != nullptr, c, d.n_vocab, row);
 }
 
-// Drafts that request b accepts: a lane of the wave for each.
+__device__ __forceinline__ StopRow stop_row(const mako_row_cut& c, uint32_t n_vocab)
+{
+    return {(double)c.max_logit, weight_scale(c.temperature), c.total > 0.0 ? 1.0 / c.total : 0.0, c.cut_logit, c.cut_token, c.n_kept < n_vocab / 64u, 0u};
+}
+template <class T>
+union Words {
+    T value;
+    int words[sizeof(T) / 4];
+};
+template <class T>
+__device__ __forceinline__ T of_lane(const T& v, uint32_t from)
+{
+    Words<T> u;
+    u.value = v;
+#pragma unroll
+    for (uint32_t k = 0; k < sizeof(T) / 4u; ++k)
+        u.words[k] = __builtin_amdgcn_readlane(u.words[k], (int)from);
+    return u.value;
+}
+
+// Where request b stops: a lane of the wave for each draft.  Everything but the drafts' own logits is asked for at once.
 template <class E, class Q>
-__device__ __forceinline__ uint32_t accepted_drafts(const mako_verify_desc& d, uint32_t b, uint32_t drafts)
+__device__ __forceinline__ Stop find_stop(const mako_verify_desc& d, uint32_t b, int32_t n_drafts)
 {
-    const uint32_t j = (uint32_t)lane();
-    bool stop = j >= drafts;
-    if (!stop) {
-        const uint32_t token = (uint32_t)d.draft_tokens[(uint64_t)b * d.max_drafts + j];
-        const double p = target_row<E>(d, (uint64_t)b * (d.max_drafts + 1) + j).one(token);
-        const double q = d.draft ? draft_row<Q>(d, (uint64_t)b * d.max_drafts + j).one(token) : 1.0;
-        stop = !((double)d.u[(uint64_t)b * (d.max_drafts + 1) + j] * q < p);
+    const uint32_t k = d.max_drafts, j = (uint32_t)lane();
+    const uint64_t p_row = (uint64_t)b * (k + 1), q_row = (uint64_t)b * k;
+    mako_row_cut p_cut = {}, q_cut = {};
+    uint32_t token = kNoToken;
+    float u = 1.0f;
+    if (j <= k && d.target_cuts)
+        p_cut = d.target_cuts[p_row + j];
+    if (j < k) {
+        token = (uint32_t)d.draft_tokens[q_row + j];
+        u = d.u[p_row + j];
+        if (d.draft && d.draft_cuts)
+            q_cut = d.draft_cuts[q_row + j];
     }
-    const unsigned long long stops = __ballot(stop);
-    return min(stops ? (uint32_t)__builtin_ctzll(stops) : 64u, drafts);
+    StopRow p_stop = stop_row(p_cut, d.n_vocab);
+    const StopRow q_stop = stop_row(q_cut, d.n_vocab);
+    const Row<E> p = target_row<E>(d, p_stop, p_row + j);
+    const Row<Q> q = draft_row<Q>(d, q_stop, q_row + j);
+    float p_logit = 0.0f, q_logit = 0.0f;
+    uint32_t p_bits = ~0u, q_bits = ~0u;
+    if (token < d.n_vocab) {
+        p_logit = E::of(p.x[token], 0);
+        if (p.mask)
+            p_bits = p.mask[token >> 5];
+        if (d.draft) {
+            q_logit = Q::of(q.x[token], 0);
+            if (q.mask)
+                q_bits = q.mask[token >> 5];
+        }
+    }
+    const uint32_t drafts = min((uint32_t)max(n_drafts, 0), k);
+    const bool stops = j >= drafts || !((double)u * (d.draft ? q.one(token, q_logit, q_bits) : 1.0) < p.one(token, p_logit, p_bits));
+    const unsigned long long all = __ballot(stops);
+    Stop stop;
+    stop.accepted = all ? (uint32_t)__builtin_ctzll(all) : 64u;
+    stop.rejected = stop.accepted < drafts;
+    const uint32_t at = min(stop.accepted, 63u);
+    stop.target = of_lane(p_stop, at);
+    stop.draft = of_lane(q_stop, at);
+    if (stop.accepted == 64u && d.target_cuts) // (as many drafts as lanes, and all are accepted)
+        stop.target = stop_row(d.target_cuts[p_row + 64u], d.n_vocab);
+    stop.without = stop.rejected && !d.draft ? (uint32_t)__builtin_amdgcn_readlane((int)token, (int)at) : kNoToken;
+    stop.reserved = 0;
+    return stop;
 }
 
 template <class E, class Q>
-__device__ __forceinline__ Left<E, Q> left_of(const mako_verify_desc& d, uint32_t b, uint32_t accepted, uint32_t drafts)
+__device__ __forceinline__ Left<E, Q> left_of(const mako_verify_desc& d, uint32_t b, const Stop& stop)
 {
-    const bool rejected = accepted < drafts;
-    const bool minus_q = rejected && d.draft;
-    Left<E, Q> left = {target_row<E>(d, (uint64_t)b * (d.max_drafts + 1) + accepted),
-                      minus_q ? draft_row<Q>(d, (uint64_t)b * d.max_drafts + accepted) : Row<Q>(nullptr, 0, nullptr, 0, nullptr, d.n_vocab, 0), minus_q, kNoToken};
-    if (rejected && !d.draft)
-        left.without = (uint32_t)d.draft_tokens[(uint64_t)b * d.max_drafts + accepted];
-    return left;
+    return {target_row<E>(d, stop.target, (uint64_t)b * (d.max_drafts + 1) + stop.accepted), draft_row<Q>(d, stop.draft, (uint64_t)b * d.max_drafts + stop.accepted),
+            stop.rejected && d.draft, stop.without};
 }
 
 template <class E, class Q>
-__global__ void __launch_bounds__(kThreads) left_kernel(mako_verify_desc d, Scratch sc)
+__global__ void __launch_bounds__(kThreads, 6) left_kernel(mako_verify_desc d, Scratch sc, uint32_t each)
 {
-    __shared__ Share<kWaves> share;
-    const uint32_t b = blockIdx.y;
-    bool there;
-    const uint32_t drafts = drafts_of(d, b, there);
-    if (!there)
+    __shared__ double sums[kMostParts][kWaves];
+    __shared__ Words<Stop> shared;
+    const uint32_t b = blockIdx.y, parts = (d.n_vocab + kPart - 1) / kPart, first = blockIdx.x * each, n = min(each, parts - first);
+    const int32_t n_drafts = d.n_drafts ? d.n_drafts[b] : (int32_t)d.max_drafts;
+    // (one wave finds the place: by all of them that alone took as long as the rest)
+    if (wave() == 0) {
+        const Stop found = find_stop<E, Q>(d, b, n_drafts);
+        if (threadIdx.x == 0) {
+            shared.value = found;
+            if (blockIdx.x == 0)
+                sc.stops[b] = found;
+        }
+    }
+    for (uint32_t k = threadIdx.x; k < kMostParts * kWaves; k += kThreads)
+        sums[k / kWaves][k % kWaves] = 0.0;
+    __syncthreads();
+    if (n_drafts < 0)
         return;
-    const uint32_t accepted = accepted_drafts<E, Q>(d, b, drafts);
-    const Left<E, Q> left = left_of<E, Q>(d, b, accepted, drafts);
-    double r[16];
-    const double sum = all_sum<kWaves>(left.slice(blockIdx.x, r), share);
-    if (threadIdx.x == 0) {
-        sc.parts[(uint64_t)b * sc.parts_cap + blockIdx.x] = sum;
-        if (blockIdx.x == 0)
-            sc.stop[b] = accepted;
+    Words<Stop> known;
+#pragma unroll
+    for (uint32_t k = 0; k < sizeof(Stop) / 4u; ++k)
+        known.words[k] = __builtin_amdgcn_readfirstlane(shared.words[k]);
+    const Left<E, Q> left = left_of<E, Q>(d, b, known.value);
+    uint32_t todo = 0xffffffffu >> (32u - n);
+    if (left.p.few) {
+        // Of a row that keeps few tokens most parts have nothing: all are looked at before anything else is asked for, four at a
+        // time.  (A masked token may be taken for one that is kept: the part is then found to have nothing.)
+        for (uint32_t j = 0; j < n; j += 4u) {
+            float v[4][4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k)
+                if (j + k < n)
+                    left.p.load((first + j + k) * kPart + threadIdx.x * 4u, (first + j + k + 1u) * kPart <= d.n_vocab, v[k]);
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                bool any = false;
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e)
+                    any = any || left.p.may_keep(v[k][e]);
+                if (j + k < n && !__ballot(any))
+                    todo &= ~(1u << (j + k));
+            }
+        }
+    }
+    if (todo) {
+        float v[4], w[4];
+        left.load(first + (uint32_t)__builtin_ctz(todo), v, w);
+#pragma unroll 1
+        while (todo) {
+            const uint32_t j = (uint32_t)__builtin_ctz(todo);
+            todo &= todo - 1u;
+            float next_v[4], next_w[4];
+            if (todo)
+                left.load(first + (uint32_t)__builtin_ctz(todo), next_v, next_w);
+            double r[4];
+            left.four(first + j, v, w, r);
+            const double sum = __ockl_wfred_add_f64(r[0] + r[1] + r[2] + r[3]);
+            if (lane() == 0)
+                sums[j][wave()] = sum;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = next_v[k];
+                w[k] = next_w[k];
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < n) {
+        double sum = 0.0;
+        for (int k = 0; k < kWaves; ++k)
+            sum += sums[threadIdx.x][k];
+        sc.parts[(uint64_t)b * sc.parts_cap + first + threadIdx.x] = sum;
     }
 }
 
@@ -181,80 +303,106 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
 {
     __shared__ Share<kWaves> share;
     __shared__ double found_before;
-    const uint32_t b = blockIdx.x, places = d.max_drafts + 1;
-    bool there;
-    const uint32_t drafts = drafts_of(d, b, there);
-    if (!there)
+    const uint32_t b = blockIdx.x, places = d.max_drafts + 1, parts = (d.n_vocab + kPart - 1) / kPart;
+    const int32_t n_drafts = d.n_drafts ? d.n_drafts[b] : 0;
+    const Stop stop = sc.stops[b]; // (of a request that is not there: not looked at)
+    // the parts: four to a thread (no more than 1024 of them)
+    static_assert(MAKO_STEP_MAX_VOCAB / kPart <= 4 * kThreads, "parts of a row");
+    double part[4], r[4], total;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; ++k)
+        part[k] = threadIdx.x * 4u + k < parts ? sc.parts[(uint64_t)b * sc.parts_cap + threadIdx.x * 4u + k] : 0.0;
+    const float u = d.u[(uint64_t)b * places + d.max_drafts];
+    int32_t draft = -1;
+    if (threadIdx.x < d.max_drafts)
+        draft = d.draft_tokens[(uint64_t)b * d.max_drafts + threadIdx.x];
+    const int32_t length = d.seq_len ? d.seq_len[b] : 0;
+    if (n_drafts < 0)
         return;
-    const uint32_t accepted = sc.stop[b];
-    Left<E, Q> left = left_of<E, Q>(d, b, accepted, drafts);
-    const uint32_t slices = (d.n_vocab + kPart - 1) / kPart;
-    double* parts = sc.parts + (uint64_t)b * sc.parts_cap;
-    double r[16];
-    // the slices: one to a thread (no more than 256 of them)
-    double part = threadIdx.x < slices ? parts[threadIdx.x] : 0.0, total;
-    double before = sum_before<kWaves>(part, total, share);
-    if (!(total > 0.0)) {
-        // nothing is left: from p itself
-        left.give_up();
-        for (uint32_t s = 0; s < slices; ++s) {
-            const double sum = all_sum<kWaves>(left.slice(s, r), share);
-            if (threadIdx.x == s)
-                part = sum;
-        }
-        before = sum_before<kWaves>(part, total, share);
-    }
+    Left<E, Q> left = left_of<E, Q>(d, b, stop);
+    double before = sum_before<kWaves>(part[0] + part[1] + part[2] + part[3], total, share);
+    // (a part whose token is drawn, and what is before it)
     uint32_t token = kNoToken;
-    if (total > 0.0) {
-        const double goal = (double)d.u[(uint64_t)b * places + d.max_drafts] * total;
-        // the first slice, then the first token, with which the running sum exceeds the goal; should rounding leave none, the
-        // last that has a weight
-        const uint32_t first = all_min<kWaves>(part > 0.0 && before + part > goal ? threadIdx.x : kNoToken, share);
-        const uint32_t last = ~all_min<kWaves>(part > 0.0 ? ~threadIdx.x : kNoToken, share);
-        const uint32_t at = first != kNoToken ? first : last;
-        if (threadIdx.x == at)
-            found_before = before;
-        __syncthreads();
-        left.slice(at, r);
-        double run = found_before;
-        uint32_t hit = kNoToken, weighty = 0; // (weighty: a token + 1)
+    bool again = false;
+    for (;;) {
+        uint32_t at = kNoToken;
+        double goal = 0.0;
+        if (total > 0.0) {
+            goal = (double)u * total;
+            // the first part, then the first token, with which the running sum exceeds the goal; should rounding leave none, the
+            // last that has a weight
+            uint32_t hit = kNoToken, last = 0;
+            double upto = before, hit_before = 0.0, last_before = 0.0;
 #pragma unroll
-        for (uint32_t j = 0; j < kRuns; ++j) {
-            const uint32_t i = at * kPart + (j * kThreads + threadIdx.x) * kRun;
-            double mine = 0.0, all;
-#pragma unroll
-            for (uint32_t k = 0; k < kRun; ++k)
-                mine += r[j * kRun + k];
-            double here = run + sum_before<kWaves>(mine, all, share);
-#pragma unroll
-            for (uint32_t k = 0; k < kRun; ++k) {
-                const double w = r[j * kRun + k];
-                here += w;
-                if (w > 0.0) {
-                    weighty = i + k + 1u;
-                    if (here > goal && hit == kNoToken)
-                        hit = i + k;
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const double from = upto;
+                upto += part[k];
+                if (part[k] > 0.0) {
+                    last = threadIdx.x * 4u + k + 1u;
+                    last_before = from;
+                    if (upto > goal && hit == kNoToken) {
+                        hit = threadIdx.x * 4u + k;
+                        hit_before = from;
+                    }
                 }
             }
-            run += all;
+            const uint32_t first = all_min<kWaves>(hit, share), behind = ~all_min<kWaves>(~last, share);
+            at = first != kNoToken ? first : behind - 1u;
+            if (first != kNoToken ? hit == first : last == behind)
+                found_before = first != kNoToken ? hit_before : last_before;
+            __syncthreads();
+        } else if (again) {
+            break;
+        }
+        if (at == kNoToken) {
+            // nothing is left: from p itself
+            left.give_up();
+            again = true;
+            for (uint32_t i = 0; i < parts; ++i) {
+                left.part(i, r);
+                const double sum = all_sum<kWaves>(r[0] + r[1] + r[2] + r[3], share);
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k)
+                    if (i == threadIdx.x * 4u + k)
+                        part[k] = sum;
+            }
+            before = sum_before<kWaves>(part[0] + part[1] + part[2] + part[3], total, share);
+            continue;
+        }
+        left.part(at, r);
+        double all;
+        double here = found_before + sum_before<kWaves>(r[0] + r[1] + r[2] + r[3], all, share);
+        uint32_t hit = kNoToken, weighty = 0; // (weighty: a token + 1)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
+            here += r[k];
+            if (r[k] > 0.0) {
+                weighty = at * kPart + threadIdx.x * 4u + k + 1u;
+                if (here > goal && hit == kNoToken)
+                    hit = weighty - 1u;
+            }
         }
         hit = all_min<kWaves>(hit, share);
         weighty = ~all_min<kWaves>(~weighty, share);
         token = hit != kNoToken ? hit : weighty - 1u;
+        break;
     }
-    for (uint32_t j = threadIdx.x; j < places; j += kThreads)
-        d.out_tokens[(uint64_t)b * places + j] = j < accepted ? d.draft_tokens[(uint64_t)b * d.max_drafts + j] : (j == accepted ? (int32_t)token : -1);
+    if (threadIdx.x < places)
+        d.out_tokens[(uint64_t)b * places + threadIdx.x] = threadIdx.x < stop.accepted ? draft : (threadIdx.x == stop.accepted ? (int32_t)token : -1);
     if (threadIdx.x == 0) {
-        d.out_accepted[b] = (int32_t)accepted;
+        d.out_accepted[b] = (int32_t)stop.accepted;
         if (d.seq_len)
-            d.out_seq_len[b] = d.seq_len[b] + (int32_t)accepted + (token != kNoToken);
+            d.out_seq_len[b] = length + (int32_t)stop.accepted + (token != kNoToken);
     }
 }
 
+constexpr uint32_t kWorkgroups = 2048;
 template <class E, class Q>
 void verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
 {
-    hipLaunchKernelGGL((left_kernel<E, Q>), dim3((d.n_vocab + kPart - 1) / kPart, d.n_requests), dim3(kThreads), 0, st, d, sc);
+    const uint32_t parts = (d.n_vocab + kPart - 1) / kPart;
+    const uint32_t each = (uint32_t)min((uint64_t)kMostParts, ((uint64_t)parts * d.n_requests + kWorkgroups - 1) / kWorkgroups);
+    hipLaunchKernelGGL((left_kernel<E, Q>), dim3((parts + each - 1) / each, d.n_requests), dim3(kThreads), 0, st, d, sc, each);
     hipLaunchKernelGGL((draw_kernel<E, Q>), dim3(d.n_requests), dim3(kThreads), 0, st, d, sc);
 }
 template <class E>

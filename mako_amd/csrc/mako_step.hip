@@ -98,7 +98,7 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     if (e == hipSuccess)
         e = take(sc.parts, rows * sc.parts_cap);
     if (e == hipSuccess)
-        e = take(sc.stop, rows);
+        e = take(sc.stops, rows);
     if (e == hipSuccess)
         e = take(sc.released, rows + 1);
     if (e == hipSuccess)
@@ -125,7 +125,7 @@ void mako_step_destroy(mako_step_ctx* ctx)
     {
         const OnDevice on(ctx->device);
         mako::step::Scratch& sc = ctx->sc;
-        void* ptrs[] = {sc.chunks, sc.lists, sc.looks, sc.plans, sc.wide, sc.parts, sc.stop, sc.released, sc.taken, sc.held, sc.free_state};
+        void* ptrs[] = {sc.chunks, sc.lists, sc.looks, sc.plans, sc.wide, sc.parts, sc.stops, sc.released, sc.taken, sc.held, sc.free_state};
         for (void* p : ptrs)
             if (p)
                 (void)hipFree(p);

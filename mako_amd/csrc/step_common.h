@@ -20,7 +20,7 @@ extern "C" __device__ uint64_t __ockl_wfscan_add_u64(uint64_t, bool inclusive);
 namespace mako {
 namespace step {
 
-constexpr uint32_t kPart = 4096;        // logits of a row that a workgroup of 256 threads takes: 16 a thread
+constexpr uint32_t kPart = 1024;        // logits of a row that a workgroup of 256 threads takes: 4 a thread
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr float kFltMax = 3.402823466e+38f;
 constexpr double kLog2e = 1.4426950408889634;
@@ -29,6 +29,7 @@ constexpr double kLog2e = 1.4426950408889634;
 // (a row may begin at any element: the loads promise no more than that)
 typedef uint32_t words_at_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t words_at_2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t pair_at_2 __attribute__((ext_vector_type(2), aligned(2)));
 struct F32 {
     using raw = uint32_t;
     using words = words_at_4;
@@ -70,6 +71,34 @@ __device__ __forceinline__ void load_vec(const void* row, uint32_t i, uint32_t n
     } else {
 #pragma unroll
         for (uint32_t k = 0; k < E::kVec; ++k) {
+            x[k] = __uint_as_float(0x7fc00000u);
+            if (i + k < n)
+                x[k] = E::of(static_cast<const typename E::raw*>(row)[i + k], 0);
+        }
+    }
+}
+
+// Four logits from i on (a multiple of four), the same way.
+template <class E>
+__device__ __forceinline__ void load_whole_four(const void* row, uint32_t i, float* x)
+{
+    if (sizeof(typename E::raw) == 4) {
+        load_whole<E>(row, i, x);
+    } else {
+        const pair_at_2 w = *reinterpret_cast<const pair_at_2*>(static_cast<const typename E::raw*>(row) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            x[k] = E::of(w[k / 2], k);
+    }
+}
+template <class E>
+__device__ __forceinline__ void load_four(const void* row, uint32_t i, uint32_t n, float* x)
+{
+    if (i + 4u <= n) {
+        load_whole_four<E>(row, i, x);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) {
             x[k] = __uint_as_float(0x7fc00000u);
             if (i + k < n)
                 x[k] = E::of(static_cast<const typename E::raw*>(row)[i + k], 0);
@@ -127,6 +156,30 @@ __device__ __forceinline__ double exp2_down(double t)
     p = fma(p, f, 0.69314718055987101);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
+}
+
+// N at once, step by step: where few waves run, a chain of fp64 operations is waited for, and N of them are no longer than one.
+template <int N>
+__device__ __forceinline__ void exp2_down(const double* t, double* out)
+{
+    constexpr double c[10] = {1.0150344092361341e-07, 1.325940551832952e-06, 1.5252984798658376e-05, 0.0001540343494852222, 0.0013333557617675399,
+                              0.0096181291920665896, 0.055504108668685152, 0.24022650695649655, 0.69314718055987101, 1.0};
+    double n[N], f[N], p[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const double low = fmax(t[k], -1100.0);
+        n[k] = rint(low);
+        f[k] = low - n[k];
+        p[k] = c[0];
+    }
+#pragma unroll
+    for (int i = 1; i < 10; ++i)
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            p[k] = fma(p[k], f[k], c[i]);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        out[k] = ldexp(p[k], (int)n[k]);
 }
 
 // log2(e) / T, for weights 2^((x - max) scale).  (T infinite: as good as 0, but 0 times an infinity would be no number.)

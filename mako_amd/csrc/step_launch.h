@@ -38,6 +38,19 @@ struct RowPlan {
     uint32_t look;       // 0: there is no guess where it lies
 };
 
+// Where a request stops accepting, and what its rows there need: a row's cut with its divisions made.
+struct StopRow {
+    double max, scale, share; // a kept token's probability is 2^((logit - max) scale) share
+    float cut;
+    int32_t cut_token;
+    uint32_t few, reserved;   // few of the row's tokens are kept
+};
+struct Stop {
+    StopRow target, draft;
+    uint32_t accepted, rejected; // drafts it accepts, and whether there is one that it does not
+    uint32_t without, reserved;  // a token that is not drawn; 0xffffffff: none
+};
+
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
     uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that
@@ -47,7 +60,7 @@ struct Scratch {
     uint32_t* wide;       // [1]: how many do
     double* parts;        // [rows][parts_cap]: what is left to draw from in each part of the row where a request stops
     uint32_t parts_cap;
-    uint32_t* stop;       // [rows] drafts a request accepts
+    Stop* stops;          // [rows]
     uint32_t* released;   // [rows + 1] blocks given back by the requests before
     uint32_t* taken;      // [rows + 1] blocks taken by the requests before
     uint32_t* held;       // [rows] blocks a request keeps before it takes any
