@@ -106,6 +106,8 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     if (e == hipSuccess)
         e = take(sc.held, rows);
     if (e == hipSuccess)
+        e = take(sc.start, rows + 1);
+    if (e == hipSuccess)
         e = take(sc.free_state, 2);
     if (e == hipSuccess)
         e = mako::step::init_cut();
@@ -125,7 +127,7 @@ void mako_step_destroy(mako_step_ctx* ctx)
     {
         const OnDevice on(ctx->device);
         mako::step::Scratch& sc = ctx->sc;
-        void* ptrs[] = {sc.chunks, sc.lists, sc.looks, sc.plans, sc.wide, sc.parts, sc.stops, sc.released, sc.taken, sc.held, sc.free_state};
+        void* ptrs[] = {sc.chunks, sc.lists, sc.looks, sc.plans, sc.wide, sc.parts, sc.stops, sc.released, sc.taken, sc.held, sc.start, sc.free_state};
         for (void* p : ptrs)
             if (p)
                 (void)hipFree(p);

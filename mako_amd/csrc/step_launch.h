@@ -64,6 +64,7 @@ struct Scratch {
     uint32_t* released;   // [rows + 1] blocks given back by the requests before
     uint32_t* taken;      // [rows + 1] blocks taken by the requests before
     uint32_t* held;       // [rows] blocks a request keeps before it takes any
+    uint32_t* start;      // [rows + 1] new tokens of the requests before
     uint32_t* free_state; // [2] blocks on the free list before the call, and after the releases
 };
 

@@ -84,6 +84,18 @@ def test_batches(ctx, n, size):
     check(ctx, s, size, 12, 9 * n, optional=False)
 
 
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 5000])
+def test_many_requests(ctx, n):
+    """Plans in LDS and in device memory."""
+    rng = np.random.default_rng(n)
+    s = batch(rng, n, 16, 6, 3 * n)
+    check(ctx, s, 16, 6, 9 * n)
+    check(ctx, s, 16, 6, 9 * n, in_place=True)
+    s = batch(rng, n, 4, 6, n // 2)
+    want = check(ctx, s, 4, 6, 3 * n, in_place=True)
+    assert (want["status"] != 0).any()
+
+
 def test_prefill_chunks(ctx):
     rng = np.random.default_rng(1)
     s = batch(rng, 40, 16, 700, 3000, longest_new=2000)
