@@ -39,7 +39,7 @@ extern "C" {
 typedef struct mako_step_ctx mako_step_ctx;
 
 /* Creates a context on HIP device `device` for rows (requests) of up to max_rows and vocabularies of up to max_vocab
- * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB); its scratch memory (1.3 bytes for every logit of the
+ * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB); its scratch memory (2.5 bytes for every logit of the
  * largest batch, and 220 a row) is allocated here. */
 #define MAKO_STEP_MAX_ROWS 65535
 #define MAKO_STEP_MAX_VOCAB 1048576

@@ -543,6 +543,13 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
         const uint32_t n_before = lds.n_before[tries], n_bins = lds.n_upto[tries] - n_before;
         if ((double)n_bins * each > 0.9 * kList)
             continue;
+        // (a rank that there is room for has all tokens up to it listed: a top_p behind it is then found among them)
+        if (plan.rank && (double)lds.n_upto[tries] * each <= 0.9 * kList) {
+            plan.high = INFINITY;
+            plan.low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
+            plan.from_above = plan.look = 1;
+            return;
+        }
         plan.high = first_bin ? bins.top - (float)((double)first_bin / (double)bins.scale) : INFINITY;
         plan.low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
         plan.from_above = plan.rank || 2u * n_before + n_bins <= samples;
@@ -857,6 +864,8 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
         Want want = {plan.rank, plan.mass};
         Cut cut = {0, 0.0, 0.0f, 0};
         double total = plan.total;
+        Bins list_bins(row.max, 1.0);
+        uint32_t listed_n = 0; // tokens in lds.list, where the cut is
         __syncthreads();
         clear_bins(lds);
         if (threadIdx.x == 0)
@@ -888,14 +897,15 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
                 if (n > 0 && n <= kList) {
                     row.set_unit(kind.sums ? total : (double)kList);
                     const float from = fminf(plan.high, row.max);
-                    const Bins bins(from, (double)from - (double)plan.low);
-                    bin_list(row, bins, n, lds);
+                    list_bins = Bins(from, (double)from - (double)plan.low);
+                    bin_list(row, list_bins, n, lds);
                     u64 all;
                     (void)sum_before<kWaves>(lds.mass[2 * threadIdx.x] + lds.mass[2 * threadIdx.x + 1], all, lds.share);
                     const double in_list = row.mass(all), before = plan.from_above ? side : total - side - in_list;
                     // (is it there?)
                     if (!(above && want.reached(above, before)) && want.reached(above + n, before + in_list))
-                        cut = cut_in_bins(row, want, bins, n, above, before, lds);
+                        cut = cut_in_bins(row, want, list_bins, n, above, before, lds);
+                    listed_n = cut.n ? n : 0u;
                 }
             }
         }
@@ -905,10 +915,15 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             cut = cut_by_division(row, want, total, plan.tokens, lds);
         }
         if (plan.rank && kind.top_p) {
-            if (!kind.sums && plan.look)
-                total = row.add_all(lds);
             want = Want{0, (double)p.top_p * cut.mass};
-            cut = cut_by_division(row, want, total, plan.tokens, lds);
+            cut.n = 0;
+            if (listed_n && plan.high == INFINITY)
+                cut = cut_in_bins(row, want, list_bins, listed_n, 0, 0.0, lds);
+            if (cut.n == 0) {
+                if (!kind.sums && total == 0.0)
+                    total = row.add_all(lds);
+                cut = cut_by_division(row, want, total, plan.tokens, lds);
+            }
         }
         store_cut(out, cut, plan.tokens);
     }

@@ -138,9 +138,8 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
             rec.low = -__ockl_wfred_max_f32(-low);
         }
         if (kind.cut && d.n_vocab > kWholeRow) {
-            // the chunk's first tokens: those not below the n-th largest of the lanes' largest; above it, where these are too
-            // many (equal ones); none, where these are too many too.  A chunk of few tokens lists them all.
-            rec.listed = rec.count <= kChunkList ? -kFltMax : nth_largest(mine, kind.list_length(chunks));
+            // The chunk's first tokens: those not below the n-th largest of the lanes' largest; above it, where these are too many
+            // (equal ones); of half as many lanes, where these are too many too.  A chunk of few tokens lists them all.
             uint64_t* list = sc.lists + at * kChunkList;
             auto take = [&](bool above) {
                 rec.n_list = 0;
@@ -156,14 +155,19 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
                     }
                 }
             };
-            take(false);
-            if (rec.n_list > kChunkList) {
+            rec.listed = INFINITY;
+            for (uint32_t n = rec.count <= kChunkList ? 64u : kind.list_length(chunks); n; n /= 2u) {
+                rec.listed = rec.count <= kChunkList ? -kFltMax : nth_largest(mine, n);
+                take(false);
+                if (rec.n_list <= kChunkList)
+                    break;
                 take(true);
-                rec.listed = key_logit(order_key(rec.listed + 0.0f) - 1u); // (all of the next larger number and above)
-                if (rec.n_list > kChunkList) {
-                    rec.n_list = 0;
-                    rec.listed = INFINITY;
+                if (rec.n_list <= kChunkList) {
+                    rec.listed = key_logit(order_key(rec.listed + 0.0f) - 1u); // (all of the next larger number and above)
+                    break;
                 }
+                rec.listed = INFINITY;
+                rec.n_list = 0;
             }
             if (rec.count <= kChunkList)
                 rec.listed = -INFINITY;

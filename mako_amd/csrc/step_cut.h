@@ -30,12 +30,13 @@ struct RowKind {
         sums = !greedy && (top_k == 0 || top_k > kListTopK);
         scale = weight_scale(p.temperature);
     }
-    // Tokens that each of a row's chunks should list: what a top_k takes of one if chance spreads its tokens (the mean, and
-    // three and a half deviations); without a top_k, enough for a narrow nucleus, and more for a min_p, which has no other way.
+    // Lanes of a chunk's 64 whose largest logit should be in its list: what a top_k takes of a chunk if chance spreads its tokens
+    // (the mean, and three and a half deviations; at most 52, whose logits and those above are some 105 tokens of 2048); without a
+    // top_k, enough for a narrow nucleus, and more for a min_p, which has no other way.
     __device__ __forceinline__ uint32_t list_length(uint32_t chunks) const
     {
         const float mean = (float)min(top_k, kListTopK) / (float)chunks;
-        return top_k && top_k <= kListTopK ? min((uint32_t)(mean + 3.5f * sqrtf(mean)) + 5u, 40u) : (min_p ? 24u : 10u);
+        return top_k && top_k <= kListTopK ? min((uint32_t)(mean + 3.5f * sqrtf(mean)) + 4u, 52u) : (min_p ? 24u : 10u);
     }
 };
 

@@ -11,8 +11,8 @@ namespace step {
 
 // A row is read in chunks of 2048 logits, a wave each.
 constexpr uint32_t kChunk = 2048;
-constexpr uint32_t kChunkList = 64; // a chunk's first tokens that are written out, at most
-constexpr uint32_t kLookList = 256; // ... and those around the row's cut
+constexpr uint32_t kChunkList = 128; // a chunk's first tokens that are written out, at most
+constexpr uint32_t kLookList = 512;  // ... and those around the row's cut
 
 // (what the second pass over a row, around its cut, finds in a chunk takes the same place: `sum` of the tokens that are weighed,
 // `count` of those above, `n_list` in the list)
