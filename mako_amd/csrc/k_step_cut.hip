@@ -93,7 +93,7 @@ struct Row {
                         f(base + a * kStep + threadIdx.x * E::kVec + k, v[a][k]);
         }
     }
-    __device__ double add_all(RowLds& lds) const
+    __device__ __forceinline__ double add_all(RowLds& lds) const
     {
         double mine = 0.0;
         each([&](uint32_t, float v) { mine += weigh(v); });
@@ -127,7 +127,7 @@ struct Bin {
     u64 mass_before;        // and their weights' units
 };
 template <class E>
-__device__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, double mass, RowLds& lds)
+__device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, double mass, RowLds& lds)
 {
     const uint32_t a = 2u * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
@@ -164,7 +164,7 @@ __device__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, dou
     return bin;
 }
 
-__device__ void sort_list(uint64_t* list, uint32_t n)
+__device__ __forceinline__ void sort_list(uint64_t* list, uint32_t n)
 {
     uint32_t size = 64;
     while (size < n)
@@ -198,7 +198,7 @@ __device__ __forceinline__ uint32_t rank_of_equals(const Want& want, uint32_t n,
 
 // The cut in a list of n tokens that holds it, behind `count` tokens of `mass` that come before.
 template <class E>
-__device__ Cut cut_in_list(const Row<E>& row, const Want& want, uint64_t* list, uint32_t n, uint32_t count, double mass, RowLds& lds)
+__device__ __forceinline__ Cut cut_in_list(const Row<E>& row, const Want& want, uint64_t* list, uint32_t n, uint32_t count, double mass, RowLds& lds)
 {
     // many equal logits (of 16 bits, most): the cut is behind so many of them, in the tokens' order
     const uint32_t key = (uint32_t)(list[0] >> 32);
@@ -317,7 +317,7 @@ __device__ Cut cut_in_list(const Row<E>& row, const Want& want, uint64_t* list, 
 
 // Bins (cleared) over lds.list's n tokens.
 template <class E>
-__device__ void bin_list(const Row<E>& row, const Bins& bins, uint32_t n, RowLds& lds)
+__device__ __forceinline__ void bin_list(const Row<E>& row, const Bins& bins, uint32_t n, RowLds& lds)
 {
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const float v = key_logit((uint32_t)(lds.list[i] >> 32));
@@ -327,7 +327,7 @@ __device__ void bin_list(const Row<E>& row, const Bins& bins, uint32_t n, RowLds
 }
 // The cut in that list, behind `count` tokens of `mass`.
 template <class E>
-__device__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins, uint32_t n, uint32_t count, double mass, RowLds& lds)
+__device__ __forceinline__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins, uint32_t n, uint32_t count, double mass, RowLds& lds)
 {
     const Bin bin = find_bin(row, want, count, mass, lds);
     if (bin.n == 0)
@@ -352,7 +352,7 @@ __device__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins
 // The cut of a row by dividing it: bins over the whole row, a crowded one by its tokens' order keys, digit by digit from the
 // top, until few enough are left to hold.  For any row, with a pass over it for every step.
 template <class E>
-__device__ Cut cut_by_division(Row<E>& row, const Want& want, double total, uint32_t tokens, RowLds& lds)
+__device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, double total, uint32_t tokens, RowLds& lds)
 {
     row.set_unit(total);
     // over four times what lies between the largest logit and the one of the mean weight
@@ -425,12 +425,16 @@ __device__ Cut cut_by_division(Row<E>& row, const Want& want, double total, uint
 
 // A guess where the cut of a row lies, by a sample of it, the first eighth of every chunk: within three deviations, and where
 // these hold too many tokens, within two.
-// (range: of logits, from the largest down, in which the cut is to be expected; plan.total: not where the cut is by rank)
+// (range: of logits, from the largest down, in which the cut is to be expected; total: not where the cut is by rank)
+struct Guess {
+    float low, high;
+    uint32_t from_above, look;
+};
 template <class E>
-__device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& lds)
+__device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, double total, uint32_t tokens, double range, RowLds& lds)
 {
     constexpr uint32_t kPer = kChunk / 8, kVecs = kPer / E::kVec, kAhead = 40 / E::kVec;
-    plan.look = 0;
+    const Guess none = {0.0f, 0.0f, 0u, 0u};
     const Bins bins(row.max, range);
     clear_bins(lds);
     __syncthreads();
@@ -454,7 +458,7 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
     const uint32_t a = 2 * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
     double w[2] = {}, sum = 0.0, squares = 0.0;
-    if (!plan.rank) {
+    if (!want.rank) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             w[k] = row.weigh(bins.top - (float)(((double)(a + k) + 0.5) / (double)bins.scale));
@@ -486,7 +490,7 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
         squares_all += lds.squares[v];
     }
     if (samples == 0)
-        return;
+        return none;
     upto += n_all;
     sum += sum_all;
     squares += squares_before;
@@ -494,13 +498,13 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
     // by mass in what the tokens behind it weigh.  (A sample that holds one of the row's few heavy tokens has both far off in the
     // bins up to it.)  The cut is behind the last bin whose end is surely before it, and in the one behind the last whose end may be
     // before it, or sooner.
-    const double each = (double)plan.tokens / (double)samples, behind_goal = plan.total - plan.mass;
+    const double each = (double)tokens / (double)samples, behind_goal = total - want.mass;
     double behind = sums - sum, var = squares_all - squares;
     uint32_t n = upto, first[2] = {}, last[2] = {};
 #pragma unroll
     for (int k = 1; k >= 0; --k) {
-        const double far = plan.rank ? (double)n * each - (double)plan.rank : behind_goal - behind * each;
-        const double dev = each * sqrt(plan.rank ? (double)n + 1.0 : fmax(var, 0.0));
+        const double far = want.rank ? (double)n * each - (double)want.rank : behind_goal - behind * each;
+        const double dev = each * sqrt(want.rank ? (double)n + 1.0 : fmax(var, 0.0));
 #pragma unroll
         for (int tries = 0; tries < 2; ++tries) {
             const double z = tries ? 2.0 : 3.0;
@@ -539,23 +543,17 @@ __device__ void guess(const Row<E>& row, double range, RowPlan& plan, RowLds& ld
     for (int tries = 0; tries < 2; ++tries) {
         const uint32_t first_bin = lds.first_bin[tries], last_bin = lds.last_bin[tries];
         if (last_bin >= kBins - 1u) // (the last bin has no lower end)
-            return;
+            return none;
         const uint32_t n_before = lds.n_before[tries], n_bins = lds.n_upto[tries] - n_before;
         if ((double)n_bins * each > 0.9 * kList)
             continue;
+        const float low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
         // (a rank that there is room for has all tokens up to it listed: a top_p behind it is then found among them)
-        if (plan.rank && (double)lds.n_upto[tries] * each <= 0.9 * kList) {
-            plan.high = INFINITY;
-            plan.low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
-            plan.from_above = plan.look = 1;
-            return;
-        }
-        plan.high = first_bin ? bins.top - (float)((double)first_bin / (double)bins.scale) : INFINITY;
-        plan.low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
-        plan.from_above = plan.rank || 2u * n_before + n_bins <= samples;
-        plan.look = 1;
-        return;
+        if (want.rank && (double)lds.n_upto[tries] * each <= 0.9 * kList)
+            return {low, INFINITY, 1u, 1u};
+        return {low, first_bin ? bins.top - (float)((double)first_bin / (double)bins.scale) : INFINITY, want.rank || 2u * n_before + n_bins <= samples, 1u};
     }
+    return none;
 }
 
 // A row's chunks together: every wave does it by itself, a lane for every 64th chunk.
@@ -813,36 +811,39 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         if (list_there && rank <= n_listed)
             cut = cut_in_bins(row, Want{rank, 0.0}, bins, n_listed, 0, 0.0, lds);
     }
-    RowPlan plan;
-    plan.rank = 0;
-    plan.mass = 0.0;
+    Want want = {0u, 0.0};
     if (cut.n == 0) {
-        plan.rank = rank;
+        want.rank = rank;
     } else if (kind.top_p) {
-        plan.mass = (double)p.top_p * cut.mass;
+        want.mass = (double)p.top_p * cut.mass;
         cut.n = 0;
         if (list_there)
-            cut = cut_in_bins(row, Want{0, plan.mass}, bins, n_listed, 0, 0.0, lds);
+            cut = cut_in_bins(row, want, bins, n_listed, 0, 0.0, lds);
     }
     if (cut.n) {
         store_cut(out, cut, c.count);
         return;
     }
     // the cut lies further down
-    plan.total = c.total;
-    plan.tokens = c.count;
-    plan.low = plan.high = 0.0f;
-    plan.from_above = plan.look = 0;
     // (where it is to be expected: within four times what lies between the largest logit and the one of the mean weight, or, where
     // that is not known, twice what the lists reach down)
     const double range = kind.sums ? 4.0 * log((double)c.count / c.total) * kLog2e / row.scale : 2.0 * ((double)row.max - (double)c.listed);
-    if ((kind.sums || plan.rank) && range > 0.0 && range < 1e30)
-        guess(row, range, plan, lds);
+    Guess where = {0.0f, 0.0f, 0u, 0u};
+    if ((kind.sums || want.rank) && range > 0.0 && range < 1e30)
+        where = guess(row, want, c.total, c.count, range, lds);
     if (threadIdx.x == 0) {
+        RowPlan& plan = sc.plans[atomicAdd(sc.wide, 1u)];
+        plan.mass = want.mass;
+        plan.total = c.total;
+        plan.rank = want.rank;
         plan.row = r;
+        plan.tokens = c.count;
         plan.max = row.max;
         plan.scale = row.scale;
-        sc.plans[atomicAdd(sc.wide, 1u)] = plan;
+        plan.low = where.low;
+        plan.high = where.high;
+        plan.from_above = where.from_above;
+        plan.look = where.look;
     }
 }
 
