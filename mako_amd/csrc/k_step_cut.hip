@@ -73,7 +73,7 @@ struct Row {
     __device__ __forceinline__ u64 units(double w) const { return (u64)rint(ldexp(w, unit)); }
     __device__ __forceinline__ double mass(u64 u) const { return ldexp((double)u, -unit); }
     // (a sum of weights up to `most` keeps below 2^63)
-    __device__ __forceinline__ void set_unit(double most) { unit = 62 - ilogb(most); }
+    __device__ __forceinline__ void set_unit(double most) { unit = 63 - __builtin_amdgcn_frexp_exp(most); }
 
     // f(token, logit) for every token of the row
     template <class F>
@@ -104,7 +104,7 @@ struct Row {
 // Bins between two logits: a function that never falls as the logit does.
 struct Bins {
     float top, scale;
-    __device__ __forceinline__ Bins(float t, double range) : top(t), scale((float)fmin((double)kBins / fmax(range, 1e-30), 1e30)) {}
+    __device__ __forceinline__ Bins(float t, float range) : top(t), scale(fminf((float)kBins / fmaxf(range, 1e-30f), 1e30f)) {}
     __device__ __forceinline__ uint32_t of(float v) const { return (uint32_t)fminf(fmaxf((top - v) * scale, 0.0f), (float)(kBins - 1u)); }
 };
 
@@ -121,13 +121,14 @@ __device__ __forceinline__ void add_to_bin(RowLds& lds, uint32_t bin, u64 units)
     atomicAdd(&lds.mass[bin], units);
 }
 
-// The first bin with which the running count and mass (behind `count` tokens that weigh `mass`) get where the cut is.
+// The first bin with which the running count and mass get where the cut is, behind `count` tokens that weigh start(units of all
+// in the bins).
 struct Bin {
     uint32_t at, before, n; // n 0: none does.  before: tokens in the bins before it
-    u64 mass_before;        // and their weights' units
+    u64 mass_before, all;   // and their weights' units, and those of all
 };
-template <class E>
-__device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, double mass, RowLds& lds)
+template <class E, class F>
+__device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, F start, RowLds& lds)
 {
     const uint32_t a = 2u * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
@@ -142,14 +143,20 @@ __device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uin
         lds.n = 0;
     __syncthreads();
     uint32_t cb = c_wave - c[0] - c[1];
-    u64 mb = m_wave - m[0] - m[1];
-    for (int w = 0; w < wave(); ++w) {
-        cb += lds.counts[w];
-        mb += lds.share.u[w];
+    u64 mb = m_wave - m[0] - m[1], all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave()) {
+            cb += lds.counts[w];
+            mb += lds.share.u[w];
+        }
+        all += lds.share.u[w];
     }
+    const double mass = start(all);
+    bool was = cb != 0 && want.reached(count + cb, mass + row.mass(mb));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        if (c[k] != 0 && want.reached(count + cb + c[k], mass + row.mass(mb + m[k])) && !(cb != 0 && want.reached(count + cb, mass + row.mass(mb)))) {
+        const bool is = want.reached(count + cb + c[k], mass + row.mass(mb + m[k]));
+        if (c[k] != 0 && is && !was) {
             lds.at = a + (uint32_t)k;
             lds.before = cb;
             lds.mass_before = mb;
@@ -157,9 +164,10 @@ __device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uin
         }
         cb += c[k];
         mb += m[k];
+        was = cb != 0 && is;
     }
     __syncthreads();
-    const Bin bin = {lds.at, lds.before, lds.n, lds.mass_before};
+    const Bin bin = {lds.at, lds.before, lds.n, lds.mass_before, all};
     __syncthreads();
     return bin;
 }
@@ -325,13 +333,10 @@ __device__ __forceinline__ void bin_list(const Row<E>& row, const Bins& bins, ui
     }
     __syncthreads();
 }
-// The cut in that list, behind `count` tokens of `mass`.
+// The cut in that list, behind `count` tokens of `mass`: in one of its bins.
 template <class E>
-__device__ __forceinline__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins, uint32_t n, uint32_t count, double mass, RowLds& lds)
+__device__ __forceinline__ Cut cut_in_bin(const Row<E>& row, const Want& want, const Bins& bins, const Bin& bin, uint32_t n, uint32_t count, double mass, RowLds& lds)
 {
-    const Bin bin = find_bin(row, want, count, mass, lds);
-    if (bin.n == 0)
-        return {0, 0.0, 0.0f, 0};
     if (bin.n > kSmall)
         return cut_in_list(row, want, lds.list, n, count, mass, lds);
     if (threadIdx.x == 0)
@@ -349,19 +354,35 @@ __device__ __forceinline__ Cut cut_in_bins(const Row<E>& row, const Want& want, 
     return cut_in_list(row, want, lds.small, bin.n, count + bin.before, mass + row.mass(bin.mass_before), lds);
 }
 
+// The cut in that list, if it is there, with nothing before it.
+template <class E>
+__device__ __forceinline__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins, uint32_t n, RowLds& lds)
+{
+    const Bin bin = find_bin(row, want, 0u, [](u64) { return 0.0; }, lds);
+    if (bin.n == 0)
+        return {0, 0.0, 0.0f, 0};
+    return cut_in_bin(row, want, bins, bin, n, 0u, 0.0, lds);
+}
+
+// The range of logits, from the largest down, in which a cut by mass is to be expected: four times what lies between the largest
+// and the one of the mean weight.
+__device__ __forceinline__ float range_of(uint32_t tokens, double total, double scale)
+{
+    return 4.0f * __builtin_amdgcn_logf((float)tokens * __builtin_amdgcn_rcpf((float)total)) / (float)fmin(scale, 1e30);
+}
+
 // The cut of a row by dividing it: bins over the whole row, a crowded one by its tokens' order keys, digit by digit from the
 // top, until few enough are left to hold.  For any row, with a pass over it for every step.
 template <class E>
 __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, double total, uint32_t tokens, RowLds& lds)
 {
     row.set_unit(total);
-    // over four times what lies between the largest logit and the one of the mean weight
-    const Bins bins(row.max, 4.0 * log((double)tokens / total) * kLog2e / row.scale);
+    const Bins bins(row.max, range_of(tokens, total, row.scale));
     clear_bins(lds);
     __syncthreads();
     row.each([&](uint32_t, float v) { add_to_bin(lds, bins.of(v), row.units(row.weigh(v))); });
     __syncthreads();
-    Bin bin = find_bin(row, want, 0, 0.0, lds);
+    Bin bin = find_bin(row, want, 0, [](u64) { return 0.0; }, lds);
     const uint32_t first = bin.at;
     uint32_t before = bin.before;
     u64 mass_before = bin.mass_before;
@@ -376,7 +397,7 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
                 add_to_bin(lds, (order_key(v) >> next) & ((1u << bits) - 1u), row.units(row.weigh(v)));
         });
         __syncthreads();
-        bin = find_bin(row, want, before, row.mass(mass_before), lds);
+        bin = find_bin(row, want, before, [&](u64) { return row.mass(mass_before); }, lds);
         prefix = (shift == 32u ? 0u : prefix << bits) | bin.at;
         before += bin.before;
         mass_before += bin.mass_before;
@@ -431,7 +452,7 @@ struct Guess {
     uint32_t from_above, look;
 };
 template <class E>
-__device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, double total, uint32_t tokens, double range, RowLds& lds)
+__device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, double total, uint32_t tokens, float range, RowLds& lds)
 {
     constexpr uint32_t kPer = kChunk / 8, kVecs = kPer / E::kVec, kAhead = 40 / E::kVec;
     const Guess none = {0.0f, 0.0f, 0u, 0u};
@@ -458,10 +479,12 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     const uint32_t a = 2 * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
     double w[2] = {}, sum = 0.0, squares = 0.0;
+    const float step = __builtin_amdgcn_rcpf(bins.scale); // (of logits, a bin)
     if (!want.rank) {
+        const float step_log2 = (float)(row.scale * (double)step);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            w[k] = row.weigh(bins.top - (float)(((double)(a + k) + 0.5) / (double)bins.scale));
+            w[k] = (double)__builtin_amdgcn_exp2f(-((float)(a + (uint32_t)k) + 0.5f) * step_log2);
             sum += w[k] * c[k];
             squares += w[k] * w[k] * c[k];
         }
@@ -498,16 +521,17 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     // by mass in what the tokens behind it weigh.  (A sample that holds one of the row's few heavy tokens has both far off in the
     // bins up to it.)  The cut is behind the last bin whose end is surely before it, and in the one behind the last whose end may be
     // before it, or sooner.
-    const double each = (double)tokens / (double)samples, behind_goal = total - want.mass;
+    const float each = (float)tokens * __builtin_amdgcn_rcpf((float)samples);
+    const double behind_goal = total - want.mass;
     double behind = sums - sum, var = squares_all - squares;
     uint32_t n = upto, first[2] = {}, last[2] = {};
 #pragma unroll
     for (int k = 1; k >= 0; --k) {
-        const double far = want.rank ? (double)n * each - (double)want.rank : behind_goal - behind * each;
-        const double dev = each * sqrt(want.rank ? (double)n + 1.0 : fmax(var, 0.0));
+        const float far = want.rank ? (float)n * each - (float)want.rank : (float)(behind_goal - behind * (double)each);
+        const float dev = each * __builtin_amdgcn_sqrtf(want.rank ? (float)n + 1.0f : (float)fmax(var, 0.0));
 #pragma unroll
         for (int tries = 0; tries < 2; ++tries) {
-            const double z = tries ? 2.0 : 3.0;
+            const float z = tries ? 2.0f : 3.0f;
             if (far < -z * dev)
                 first[tries] = max(first[tries], a + (uint32_t)k + 1u);
             if (far < z * dev)
@@ -545,13 +569,13 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
         if (last_bin >= kBins - 1u) // (the last bin has no lower end)
             return none;
         const uint32_t n_before = lds.n_before[tries], n_bins = lds.n_upto[tries] - n_before;
-        if ((double)n_bins * each > 0.9 * kList)
+        if ((float)n_bins * each > 0.9f * kList)
             continue;
-        const float low = bins.top - (float)((double)(last_bin + 1u) / (double)bins.scale);
+        const float low = bins.top - (float)(last_bin + 1u) * step;
         // (a rank that there is room for has all tokens up to it listed: a top_p behind it is then found among them)
-        if (want.rank && (double)lds.n_upto[tries] * each <= 0.9 * kList)
+        if (want.rank && (float)lds.n_upto[tries] * each <= 0.9f * kList)
             return {low, INFINITY, 1u, 1u};
-        return {low, first_bin ? bins.top - (float)((double)first_bin / (double)bins.scale) : INFINITY, want.rank || 2u * n_before + n_bins <= samples, 1u};
+        return {low, first_bin ? bins.top - (float)first_bin * step : INFINITY, want.rank || 2u * n_before + n_bins <= samples, 1u};
     }
     return none;
 }
@@ -771,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     // (weights' units: by the total, or, where it is not known, by the most that the list can weigh)
     row.set_unit(kind.sums ? c.total : (double)max(n_listed, 1u));
     // (a list of all the row's tokens: the bins go as far down as weights matter)
-    const Bins bins(row.max, c.listed > -INFINITY ? (double)row.max - (double)c.listed : 64.0 / row.scale);
+    const Bins bins(row.max, c.listed > -INFINITY ? row.max - c.listed : (float)(64.0 / row.scale));
     uint32_t rank = kind.top_k ? min(c.count, kind.top_k) : c.count;
     bool all_weighty = !kind.min_p; // (or it is known how many are)
     if (list_there) {
@@ -809,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     } else {
         cut.n = 0;
         if (list_there && rank <= n_listed)
-            cut = cut_in_bins(row, Want{rank, 0.0}, bins, n_listed, 0, 0.0, lds);
+            cut = cut_in_bins(row, Want{rank, 0.0}, bins, n_listed, lds);
     }
     Want want = {0u, 0.0};
     if (cut.n == 0) {
@@ -818,18 +842,17 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         want.mass = (double)p.top_p * cut.mass;
         cut.n = 0;
         if (list_there)
-            cut = cut_in_bins(row, want, bins, n_listed, 0, 0.0, lds);
+            cut = cut_in_bins(row, want, bins, n_listed, lds);
     }
     if (cut.n) {
         store_cut(out, cut, c.count);
         return;
     }
     // the cut lies further down
-    // (where it is to be expected: within four times what lies between the largest logit and the one of the mean weight, or, where
-    // that is not known, twice what the lists reach down)
-    const double range = kind.sums ? 4.0 * log((double)c.count / c.total) * kLog2e / row.scale : 2.0 * ((double)row.max - (double)c.listed);
+    // (where the weights' sum is not known, it is to be expected within twice what the lists reach down)
+    const float range = kind.sums ? range_of(c.count, c.total, row.scale) : 2.0f * (row.max - c.listed);
     Guess where = {0.0f, 0.0f, 0u, 0u};
-    if ((kind.sums || want.rank) && range > 0.0 && range < 1e30)
+    if ((kind.sums || want.rank) && range > 0.0f && range < 1e30f)
         where = guess(row, want, c.total, c.count, range, lds);
     if (threadIdx.x == 0) {
         RowPlan& plan = sc.plans[atomicAdd(sc.wide, 1u)];
@@ -842,6 +865,8 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         plan.scale = row.scale;
         plan.low = where.low;
         plan.high = where.high;
+        plan.top_p = kind.top_p ? p.top_p : 1.0f;
+        plan.sums = kind.sums;
         plan.from_above = where.from_above;
         plan.look = where.look;
     }
@@ -852,30 +877,30 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
 {
     extern __shared__ unsigned char dyn[];
     RowLds& lds = *reinterpret_cast<RowLds*>(dyn);
-    const uint32_t rows = *sc.wide, chunks = chunks_of(d.n_vocab);
-    for (uint32_t i = blockIdx.x; i < rows; i += gridDim.x) {
+    const uint32_t chunks = chunks_of(d.n_vocab);
+    for (uint32_t i = blockIdx.x; i < d.n_rows; i += gridDim.x) {
+        // (what the pass around the cut found is asked for with the plan, before it is known that there is one)
+        const ChunkRec* recs = sc.chunks + (uint64_t)i * sc.chunks_cap;
+        const uint64_t* lists = sc.looks + (uint64_t)i * sc.chunks_cap * kLookList;
+        Chunks c;
+        LookLists listed;
+        c.load(recs, chunks);
+        listed.load(lists, chunks);
         const RowPlan plan = sc.plans[i];
-        const uint32_t r = plan.row;
-        const ChunkRec* recs = sc.chunks + (uint64_t)r * sc.chunks_cap;
-        const uint64_t* lists = sc.looks + (uint64_t)r * sc.chunks_cap * kLookList;
-        const mako_sampling_params p = d.params[r / d.rows_per_params];
-        const RowKind kind(p);
-        mako_row_cut& out = d.out_cuts[r];
-        Row<E> row(d, r, plan.max, plan.scale);
+        if (i >= *sc.wide)
+            return;
+        mako_row_cut& out = d.out_cuts[plan.row];
+        Row<E> row(d, plan.row, plan.max, plan.scale);
         Want want = {plan.rank, plan.mass};
         Cut cut = {0, 0.0, 0.0f, 0};
         double total = plan.total;
-        Bins list_bins(row.max, 1.0);
+        Bins list_bins(row.max, 1.0f);
         uint32_t listed_n = 0; // tokens in lds.list, where the cut is
         __syncthreads();
         clear_bins(lds);
         if (threadIdx.x == 0)
             lds.n = 0;
         if (plan.look) {
-            Chunks c;
-            LookLists listed;
-            c.load(recs, chunks);
-            listed.load(lists, chunks);
             double side = 0.0;
             uint32_t above = 0;
             bool room = true;
@@ -896,32 +921,31 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
                 __syncthreads();
                 const uint32_t n = listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
                 if (n > 0 && n <= kList) {
-                    row.set_unit(kind.sums ? total : (double)kList);
+                    row.set_unit(plan.sums ? total : (double)kList);
                     const float from = fminf(plan.high, row.max);
-                    list_bins = Bins(from, (double)from - (double)plan.low);
+                    list_bins = Bins(from, from - plan.low);
                     bin_list(row, list_bins, n, lds);
-                    u64 all;
-                    (void)sum_before<kWaves>(lds.mass[2 * threadIdx.x] + lds.mass[2 * threadIdx.x + 1], all, lds.share);
-                    const double in_list = row.mass(all), before = plan.from_above ? side : total - side - in_list;
+                    auto before = [&](u64 all) { return plan.from_above ? side : total - side - row.mass(all); };
+                    const Bin bin = find_bin(row, want, above, before, lds);
                     // (is it there?)
-                    if (!(above && want.reached(above, before)) && want.reached(above + n, before + in_list))
-                        cut = cut_in_bins(row, want, list_bins, n, above, before, lds);
+                    if (bin.n && !(above && want.reached(above, before(bin.all))))
+                        cut = cut_in_bin(row, want, list_bins, bin, n, above, before(bin.all), lds);
                     listed_n = cut.n ? n : 0u;
                 }
             }
         }
         if (cut.n == 0) {
-            if (!kind.sums)
+            if (!plan.sums)
                 total = row.add_all(lds);
             cut = cut_by_division(row, want, total, plan.tokens, lds);
         }
-        if (plan.rank && kind.top_p) {
-            want = Want{0, (double)p.top_p * cut.mass};
+        if (plan.rank && plan.top_p < 1.0f) {
+            want = Want{0, (double)plan.top_p * cut.mass};
             cut.n = 0;
             if (listed_n && plan.high == INFINITY)
-                cut = cut_in_bins(row, want, list_bins, listed_n, 0, 0.0, lds);
+                cut = cut_in_bins(row, want, list_bins, listed_n, lds);
             if (cut.n == 0) {
-                if (!kind.sums && total == 0.0)
+                if (!plan.sums && total == 0.0)
                     total = row.add_all(lds);
                 cut = cut_by_division(row, want, total, plan.tokens, lds);
             }

@@ -189,10 +189,14 @@ __global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch s
 {
     constexpr int kEach = 16; // (a chunk in two halves: the more waves, the less they wait for)
     __shared__ float weighed[4][64 * kEach];
-    const uint32_t chunks = chunks_of(d.n_vocab), groups = (chunks + 3) / 4, items = *sc.wide * groups;
-    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const RowPlan& plan = sc.plans[item / groups];
-        const uint32_t row = plan.row, chunk = item % groups * 4u + (uint32_t)wave();
+    const uint32_t chunks = chunks_of(d.n_vocab), groups = (chunks + 3) / 4;
+    for (uint32_t item = blockIdx.x; item < d.n_rows * groups; item += gridDim.x) {
+        // (the plan is asked for before it is known that there is one)
+        const uint32_t at_plan = item / groups, chunk = item % groups * 4u + (uint32_t)wave();
+        const RowPlan plan = sc.plans[at_plan];
+        if (at_plan >= *sc.wide)
+            return;
+        const uint32_t row = plan.row;
         const float low = plan.low, high = plan.high, max = plan.max;
         const double scale = plan.scale;
         const bool from_above = plan.from_above;
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch s
         ChunkRec rec = {0.0, 0.0f, 0.0f, 0u, 0u, 0u, 0.0f};
         // (what is weighed moves together first: where it is one logit in ten, nearly every 64 have one)
         float* const mine = weighed[wave()];
-        const uint64_t at = (uint64_t)row * sc.chunks_cap + chunk;
+        const uint64_t at = (uint64_t)at_plan * sc.chunks_cap + chunk;
         uint64_t* list = sc.looks + at * kLookList;
         double sum = 0.0;
 #pragma unroll 1

@@ -28,13 +28,15 @@ struct ChunkRec {
 
 // A row whose cut lies further down than the chunks' lists: what the second pass looks for.
 struct RowPlan {
-    double mass, total; // the cut is behind the first tokens that weigh `mass`, of all that weigh `total` (0: not known),
+    double mass, total; // the cut is behind the first tokens that weigh `mass`, of all that weigh `total` (if that is known),
     uint32_t rank;      // or, if not 0, behind the first `rank`
     uint32_t row, tokens; // which row, and how many tokens it has
     float max;          // its largest logit
     double scale;       // log2(e) / T
     float low, high;    // the tokens from `low` up to `high` are listed,
     uint32_t from_above; // those above are weighed, or those below
+    float top_p;        // of what the first `rank` weigh; 1: none
+    uint32_t sums;      // `total` is known
     uint32_t look;       // 0: there is no guess where it lies
 };
 
@@ -54,7 +56,7 @@ struct Stop {
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
     uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that
-    uint64_t* looks;      // [rows][chunks_cap][kLookList]
+    uint64_t* looks;      // [rows][chunks_cap][kLookList]: by plan (and the chunks too, then)
     uint32_t chunks_cap;  // of a row
     RowPlan* plans;       // [rows]: of those that have one, in no order
     uint32_t* wide;       // [1]: how many do
