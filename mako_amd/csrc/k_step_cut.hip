@@ -879,16 +879,16 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
     RowLds& lds = *reinterpret_cast<RowLds*>(dyn);
     const uint32_t chunks = chunks_of(d.n_vocab);
     for (uint32_t i = blockIdx.x; i < d.n_rows; i += gridDim.x) {
-        // (what the pass around the cut found is asked for with the plan, before it is known that there is one)
+        const RowPlan plan = sc.plans[i];
+        if (i >= *sc.wide)
+            return;
+        // (what the pass around the cut found is asked for before the plan is there)
         const ChunkRec* recs = sc.chunks + (uint64_t)i * sc.chunks_cap;
         const uint64_t* lists = sc.looks + (uint64_t)i * sc.chunks_cap * kLookList;
         Chunks c;
         LookLists listed;
         c.load(recs, chunks);
         listed.load(lists, chunks);
-        const RowPlan plan = sc.plans[i];
-        if (i >= *sc.wide)
-            return;
         mako_row_cut& out = d.out_cuts[plan.row];
         Row<E> row(d, plan.row, plan.max, plan.scale);
         Want want = {plan.rank, plan.mass};
@@ -954,7 +954,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
     }
 }
 
-constexpr uint32_t kProbs = 4096; // logits of a workgroup
+constexpr uint32_t kProbs = 2048; // logits of a workgroup (of 128 rows of 32000 it takes 9.4 us; 1024: 9.6; 4096, with a branch for each logit: 10.5)
 template <class E>
 __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
 {
@@ -964,28 +964,47 @@ __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
     const uint32_t* mask = d.mask ? d.mask + (int64_t)r * d.mask_stride : nullptr;
     float* out = d.out_probs + (int64_t)r * d.probs_stride;
     const double scale = weight_scale(c.temperature), md = (double)c.max_logit, share = c.total > 0.0 ? 1.0 / c.total : 0.0;
-    for (uint32_t j = 0; j < 16u / E::kVec; ++j) {
-        const uint32_t i = blockIdx.x * kProbs + (j * 256u + threadIdx.x) * E::kVec;
+    // (all of a thread's logits asked for before the first is used; four at a time, so that a wave's stores leave no gaps)
+    constexpr uint32_t kFours = kProbs / 1024u;
+    const uint32_t first = blockIdx.x * kProbs + threadIdx.x * 4u;
+    float x[kFours][4];
+#pragma unroll
+    for (uint32_t j = 0; j < kFours; ++j) {
+        const uint32_t i = first + j * 1024u;
+        load_four<E>(x_row, i, d.n_vocab, x[j]);
+        const uint32_t bits = !mask ? 0xfu : (i < d.n_vocab ? mask[i >> 5] >> (i & 31u) : 0u);
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k)
+            x[j][k] = token_logit(x[j][k], (bits >> k) & 1u);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kFours; ++j) {
+        const uint32_t i = first + j * 1024u;
         if (i >= d.n_vocab)
             break;
-        float x[E::kVec], p[E::kVec];
-        load_tokens<E>(x_row, mask, i, d.n_vocab, x);
+        float p[4] = {};
+        bool kept[4], any = false;
 #pragma unroll
-        for (uint32_t k = 0; k < E::kVec; ++k) {
-            const bool kept = x[k] > c.cut_logit || (x[k] == c.cut_logit && (int32_t)(i + k) <= c.cut_token);
-            p[k] = 0.0f;
-            if (__ballot(kept))
-                p[k] = kept ? (float)(weight(x[k], md, scale) * share) : 0.0f;
+        for (uint32_t k = 0; k < 4u; ++k) {
+            kept[k] = x[j][k] > c.cut_logit || (x[j][k] == c.cut_logit && (int32_t)(i + k) <= c.cut_token);
+            any = any || kept[k];
         }
-        if (i + E::kVec <= d.n_vocab) {
+        if (__ballot(any)) {
+            double t[4], w[4];
 #pragma unroll
-            for (uint32_t k = 0; k < E::kVec; k += 4u) {
-                const words_at_4 w = {__float_as_uint(p[k]), __float_as_uint(p[k + 1]), __float_as_uint(p[k + 2]), __float_as_uint(p[k + 3])};
-                *reinterpret_cast<words_at_4*>(out + i + k) = w;
-            }
+            for (uint32_t k = 0; k < 4u; ++k)
+                t[k] = ((double)x[j][k] - md) * scale;
+            exp2_down<4>(t, w);
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k)
+                p[k] = kept[k] ? (float)(w[k] * share) : 0.0f;
+        }
+        if (i + 4u <= d.n_vocab) {
+            const words_at_4 w = {__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
+            *reinterpret_cast<words_at_4*>(out + i) = w;
         } else {
 #pragma unroll
-            for (uint32_t k = 0; k < E::kVec; ++k)
+            for (uint32_t k = 0; k < 4u; ++k)
                 if (i + k < d.n_vocab)
                     out[i + k] = p[k];
         }
@@ -998,6 +1017,8 @@ void cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
     launch_scan(st, d, sc);
     hipLaunchKernelGGL(row_kernel<E>, dim3(d.n_rows), dim3(kThreads), sizeof(RowLds), st, d, sc);
+    if (d.n_vocab <= kWholeRow)
+        return; // (every row's tokens are listed: its cut is found there)
     launch_look(st, d, sc);
     hipLaunchKernelGGL(wide_kernel<E>, dim3(d.n_rows < kWideWorkgroups ? d.n_rows : kWideWorkgroups), dim3(kThreads), sizeof(RowLds), st, d, sc);
 }
