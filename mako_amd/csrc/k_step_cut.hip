@@ -642,7 +642,7 @@ struct Chunks {
 template <uint32_t kSlots, uint32_t kRoom, uint32_t kAhead>
 struct Lists {
     static constexpr uint32_t kOfWave = 64 / kSlots, kOfAll = kOfWave * kWaves; // chunks of a load
-    static_assert(kOfAll <= 64 && kAhead * kOfAll <= kHeld * 64u, "chunks that are in registers");
+    static_assert(kOfAll <= 64 && kAhead * kOfAll <= kHeld * 64u && kHeld == 2 && kAhead >= 4, "chunks that are in registers");
     uint64_t entry[kAhead];
 
     static __device__ __forceinline__ uint32_t chunk(uint32_t a) { return a * kOfAll + (uint32_t)wave() * kOfWave + (uint32_t)lane() / kSlots; }
@@ -685,28 +685,51 @@ struct Lists {
             put(entry[a], in[a] >> lane() & 1ull, at + (uint32_t)__popcll(in[a] & before));
             at += (uint32_t)__popcll(in[a]);
         }
-        // longer lists, and the chunks beyond
-        auto rest = [&](uint32_t i, uint32_t slot, uint32_t of_chunk) {
-            for (; slot < of_chunk; slot += 64u) {
-                const uint64_t e = slot + (uint32_t)lane() < of_chunk ? lists[i * kRoom + slot + (uint32_t)lane()] : 0ull;
-                const bool in_list = slot + (uint32_t)lane() < of_chunk && __uint_as_float((uint32_t)(e >> 32)) >= from;
-                const u64 more = __ballot(in_list);
-                uint32_t to = 0;
-                if (lane() == 0 && more)
-                    to = atomicAdd(&lds.n, (uint32_t)__popcll(more));
-                to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
-                put(e, in_list, to + (uint32_t)__popcll(more & before));
-            }
-        };
+        // longer lists, and the chunks beyond: every wave those of every eighth chunk, of four of them at a time
+        constexpr uint32_t kHeldChunks = kAhead * kOfAll, kBatch = 4;
+        if (chunks > kHeldChunks || __ballot(c.rec[0].n_list > kSlots || c.rec[1].n_list > kSlots))
+            for (uint32_t base = (uint32_t)wave(); base < chunks; base += kWaves * kBatch) {
+                uint32_t of_chunk[kBatch], slot[kBatch];
+                bool more = false;
 #pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h)
-            for (u64 left = __ballot(c.rec[h].n_list > kSlots); left; left &= left - 1u) {
-                const uint32_t i = (uint32_t)__builtin_ctzll(left);
-                if (i % kWaves == (uint32_t)wave() && h * 64u + i < kAhead * kOfAll)
-                    rest(h * 64u + i, kSlots, (uint32_t)__builtin_amdgcn_readlane((int)c.rec[h].n_list, (int)i));
+                for (uint32_t a = 0; a < kBatch; ++a) {
+                    const uint32_t i = base + a * kWaves;
+                    of_chunk[a] = 0;
+                    if (i < 64u * kHeld)
+                        of_chunk[a] = (uint32_t)__builtin_amdgcn_readlane((int)(i < 64u ? c.rec[0].n_list : c.rec[1].n_list), (int)(i & 63u));
+                    else if (i < chunks)
+                        of_chunk[a] = recs[i].n_list;
+                    slot[a] = i < kHeldChunks ? kSlots : 0u;
+                    more = more || slot[a] < of_chunk[a];
+                }
+                while (more) {
+                    uint64_t e[kBatch];
+                    uint32_t m = 0;
+                    more = false;
+#pragma unroll
+                    for (uint32_t a = 0; a < kBatch; ++a) {
+                        e[a] = (uint64_t)__float_as_uint(-INFINITY) << 32;
+                        if (slot[a] + (uint32_t)lane() < of_chunk[a])
+                            e[a] = lists[(base + a * kWaves) * kRoom + slot[a] + (uint32_t)lane()];
+                    }
+#pragma unroll
+                    for (uint32_t a = 0; a < kBatch; ++a) {
+                        in[a] = __ballot(slot[a] + (uint32_t)lane() < of_chunk[a] && __uint_as_float((uint32_t)(e[a] >> 32)) >= from);
+                        m += (uint32_t)__popcll(in[a]);
+                        slot[a] += 64u;
+                        more = more || slot[a] < of_chunk[a];
+                    }
+                    at = 0;
+                    if (lane() == 0 && m)
+                        at = atomicAdd(&lds.n, m);
+                    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+#pragma unroll
+                    for (uint32_t a = 0; a < kBatch; ++a) {
+                        put(e[a], in[a] >> lane() & 1ull, at + (uint32_t)__popcll(in[a] & before));
+                        at += (uint32_t)__popcll(in[a]);
+                    }
+                }
             }
-        for (uint32_t i = kAhead * kOfAll + (uint32_t)wave(); i < chunks; i += kWaves)
-            rest(i, 0u, recs[i].n_list);
         __syncthreads();
         const uint32_t all = lds.n;
         __syncthreads();
@@ -744,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     if (!whole)
         listed.load(lists, chunks);
     const mako_sampling_params p = d.params[r / d.rows_per_params];
-    const RowKind kind(p);
+    const RowKind kind(p, d.n_vocab);
     if (kind.cut) {
         clear_bins(lds);
         if (threadIdx.x == 0) {
@@ -849,8 +872,8 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
         return;
     }
     // the cut lies further down
-    // (where the weights' sum is not known, it is to be expected within twice what the lists reach down)
-    const float range = kind.sums ? range_of(c.count, c.total, row.scale) : 2.0f * (row.max - c.listed);
+    // (a cut by rank may be far from where the weight is: twice what the lists reach down)
+    const float range = fmaxf(kind.sums ? range_of(c.count, c.total, row.scale) : 0.0f, want.rank ? 2.0f * (row.max - c.listed) : 0.0f);
     Guess where = {0.0f, 0.0f, 0u, 0u};
     if ((kind.sums || want.rank) && range > 0.0f && range < 1e30f)
         where = guess(row, want, c.total, c.count, range, lds);

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
     constexpr int kEach = kChunk / 64;
     Logits<E, kEach> c(d, row, chunk * kChunk);
     const float(&x)[kEach] = c.x;
-    const RowKind kind(d.params[row / d.rows_per_params]);
+    const RowKind kind(d.params[row / d.rows_per_params], d.n_vocab);
     float mine = x[0], low = x[0];
 #pragma unroll
     for (int k = 1; k < kEach; ++k) {

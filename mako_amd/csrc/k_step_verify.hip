@@ -20,14 +20,14 @@ struct Row {
     const typename E::raw* x;
     const uint32_t* mask;
     uint32_t n;
-    bool probs, few;
+    bool probs;
     float cut;
     int32_t cut_token;
     double max, scale, share;
 
     __device__ __forceinline__ Row(const void* base, int64_t stride, const uint32_t* masks, int64_t mask_stride, bool cuts, const StopRow& c, uint32_t n_vocab, uint64_t row)
         : x(static_cast<const typename E::raw*>(base) + (int64_t)row * stride), mask(cuts && masks ? masks + (int64_t)row * mask_stride : nullptr), n(n_vocab),
-          probs(!cuts), few(c.few), cut(c.cut), cut_token(c.cut_token), max(c.max), scale(c.scale), share(c.share)
+          probs(!cuts), cut(c.cut), cut_token(c.cut_token), max(c.max), scale(c.scale), share(c.share)
     {
     }
     // Whether a logit as it is in memory can be one of a kept token; probabilities: whether it is one.
@@ -144,9 +144,9 @@ __device__ __forceinline__ Row<E> draft_row(const mako_verify_desc& d, const Sto
     return Row<E>(d.draft, d.draft_stride, d.draft_mask, d.draft_mask_stride, d.draft_cuts != nullptr, c, d.n_vocab, row);
 }
 
-__device__ __forceinline__ StopRow stop_row(const mako_row_cut& c, uint32_t n_vocab)
+__device__ __forceinline__ StopRow stop_row(const mako_row_cut& c)
 {
-    return {(double)c.max_logit, weight_scale(c.temperature), c.total > 0.0 ? 1.0 / c.total : 0.0, c.cut_logit, c.cut_token, c.n_kept < n_vocab / 64u, 0u};
+    return {(double)c.max_logit, weight_scale(c.temperature), c.total > 0.0 ? 1.0 / c.total : 0.0, c.cut_logit, c.cut_token};
 }
 template <class T>
 union Words {
@@ -181,8 +181,8 @@ __device__ __forceinline__ Stop find_stop(const mako_verify_desc& d, uint32_t b,
         if (d.draft && d.draft_cuts)
             q_cut = d.draft_cuts[q_row + j];
     }
-    StopRow p_stop = stop_row(p_cut, d.n_vocab);
-    const StopRow q_stop = stop_row(q_cut, d.n_vocab);
+    StopRow p_stop = stop_row(p_cut);
+    const StopRow q_stop = stop_row(q_cut);
     const Row<E> p = target_row<E>(d, p_stop, p_row + j);
     const Row<Q> q = draft_row<Q>(d, q_stop, q_row + j);
     float p_logit = 0.0f, q_logit = 0.0f;
@@ -207,7 +207,7 @@ __device__ __forceinline__ Stop find_stop(const mako_verify_desc& d, uint32_t b,
     stop.target = of_lane(p_stop, at);
     stop.draft = of_lane(q_stop, at);
     if (stop.accepted == 64u && d.target_cuts) // (as many drafts as lanes, and all are accepted)
-        stop.target = stop_row(d.target_cuts[p_row + 64u], d.n_vocab);
+        stop.target = stop_row(d.target_cuts[p_row + 64u]);
     stop.without = stop.rejected && !d.draft ? (uint32_t)__builtin_amdgcn_readlane((int)token, (int)at) : kNoToken;
     stop.reserved = 0;
     return stop;
@@ -236,8 +236,6 @@ __global__ void __launch_bounds__(kThreads, 6) left_kernel(mako_verify_desc d, S
                 sc.stops[b] = found;
         }
     }
-    for (uint32_t k = threadIdx.x; k < kMostParts * kWaves; k += kThreads)
-        sums[k / kWaves][k % kWaves] = 0.0;
     __syncthreads();
     if (n_drafts < 0)
         return;
@@ -246,47 +244,23 @@ __global__ void __launch_bounds__(kThreads, 6) left_kernel(mako_verify_desc d, S
     for (uint32_t k = 0; k < sizeof(Stop) / 4u; ++k)
         known.words[k] = __builtin_amdgcn_readfirstlane(shared.words[k]);
     const Left<E, Q> left = left_of<E, Q>(d, b, known.value);
-    uint32_t todo = 0xffffffffu >> (32u - n);
-    if (left.p.few) {
-        // Of a row that keeps few tokens most parts have nothing: all are looked at before anything else is asked for, four at a
-        // time.  (A masked token may be taken for one that is kept: the part is then found to have nothing.)
-        for (uint32_t j = 0; j < n; j += 4u) {
-            float v[4][4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k)
-                if (j + k < n)
-                    left.p.load((first + j + k) * kPart + threadIdx.x * 4u, (first + j + k + 1u) * kPart <= d.n_vocab, v[k]);
-#pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) {
-                bool any = false;
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e)
-                    any = any || left.p.may_keep(v[k][e]);
-                if (j + k < n && !__ballot(any))
-                    todo &= ~(1u << (j + k));
-            }
-        }
-    }
-    if (todo) {
-        float v[4], w[4];
-        left.load(first + (uint32_t)__builtin_ctz(todo), v, w);
+    // (a part's loads are on their way while the part before it is added up)
+    float v[4], w[4];
+    left.load(first, v, w);
 #pragma unroll 1
-        while (todo) {
-            const uint32_t j = (uint32_t)__builtin_ctz(todo);
-            todo &= todo - 1u;
-            float next_v[4], next_w[4];
-            if (todo)
-                left.load(first + (uint32_t)__builtin_ctz(todo), next_v, next_w);
-            double r[4];
-            left.four(first + j, v, w, r);
-            const double sum = __ockl_wfred_add_f64(r[0] + r[1] + r[2] + r[3]);
-            if (lane() == 0)
-                sums[j][wave()] = sum;
+    for (uint32_t j = 0; j < n; ++j) {
+        float next_v[4], next_w[4];
+        if (j + 1u < n)
+            left.load(first + j + 1u, next_v, next_w);
+        double r[4];
+        left.four(first + j, v, w, r);
+        const double sum = __ockl_wfred_add_f64(r[0] + r[1] + r[2] + r[3]);
+        if (lane() == 0)
+            sums[j][wave()] = sum;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[k] = next_v[k];
-                w[k] = next_w[k];
-            }
+        for (int k = 0; k < 4; ++k) {
+            v[k] = next_v[k];
+            w[k] = next_w[k];
         }
     }
     __syncthreads();

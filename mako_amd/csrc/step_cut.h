@@ -7,36 +7,41 @@
 namespace mako {
 namespace step {
 
-// Largest top_k that is looked for in the chunks' lists.
-constexpr uint32_t kListTopK = 1024;
-
 // Rows of no more logits than this are held whole where they are cut, and have no lists.
 constexpr uint32_t kWholeRow = 6144;
+
+// Largest top_k that is looked for in the chunks' lists, of a row and of a chunk's share of it.
+constexpr uint32_t kListTopK = 2500, kListShare = 32;
 
 struct RowKind {
     bool greedy, cut; // cut: something may be cut off it, and the chunks' first tokens are wanted
     bool min_p, top_p;
-    bool sums;        // the weights' sums are wanted (not where a top_k leaves few tokens: these are added up alone)
+    bool listed;      // the first top_k tokens are to be expected in the lists
+    bool sums;        // the weights' sums are wanted (not of those: they are added up alone)
     uint32_t top_k;
     double scale;     // of weights: log2(e) / T
 
-    __device__ __forceinline__ explicit RowKind(const mako_sampling_params& p)
+    __device__ __forceinline__ RowKind(const mako_sampling_params& p, uint32_t n_vocab)
     {
         greedy = !(p.temperature > 0.0f);
         min_p = !greedy && p.min_p > 0.0f;
         top_p = !greedy && p.top_p < 1.0f;
         top_k = greedy ? 0u : p.top_k;
         cut = min_p || top_p || top_k;
-        sums = !greedy && (top_k == 0 || top_k > kListTopK);
+        listed = top_k && top_k < n_vocab && (n_vocab <= kWholeRow || top_k <= min(kListTopK, kListShare * chunks_of(n_vocab)));
+        sums = !greedy && !listed;
         scale = weight_scale(p.temperature);
     }
-    // Lanes of a chunk's 64 whose largest logit should be in its list: what a top_k takes of a chunk if chance spreads its tokens
-    // (the mean, and three and a half deviations; at most 52, whose logits and those above are some 105 tokens of 2048); without a
-    // top_k, enough for a narrow nucleus, and more for a min_p, which has no other way.
+    // Lanes of a chunk's 64 whose largest logit should be in its list.  What a top_k takes of a chunk if chance spreads its tokens, the
+    // mean and some four deviations and three, and a fifth of that again for how chance spreads them over the lanes: t tokens leave
+    // 64 exp(-t / 64) lanes without one (t is 71 at most, well below the 128 that there is room for).  Without such a top_k,
+    // enough for a narrow nucleus, and more for a min_p, which has no other way.
     __device__ __forceinline__ uint32_t list_length(uint32_t chunks) const
     {
-        const float mean = (float)min(top_k, kListTopK) / (float)chunks;
-        return top_k && top_k <= kListTopK ? min((uint32_t)(mean + 3.5f * sqrtf(mean)) + 4u, 52u) : (min_p ? 24u : 10u);
+        if (!listed)
+            return min_p ? 24u : 10u;
+        const float mean = (float)top_k / (float)chunks, t = 1.2f * (mean + 4.2f * sqrtf(mean) + 3.0f);
+        return (uint32_t)(65.0f - 64.0f * __builtin_amdgcn_exp2f(-(1.4426950f / 64.0f) * t));
     }
 };
 

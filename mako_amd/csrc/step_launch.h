@@ -45,7 +45,6 @@ struct StopRow {
     double max, scale, share; // a kept token's probability is 2^((logit - max) scale) share
     float cut;
     int32_t cut_token;
-    uint32_t few, reserved;   // few of the row's tokens are kept
 };
 struct Stop {
     StopRow target, draft;
