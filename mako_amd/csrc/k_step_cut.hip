@@ -380,7 +380,23 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
     const Bins bins(row.max, range_of(tokens, total, row.scale));
     clear_bins(lds);
     __syncthreads();
-    row.each([&](uint32_t, float v) { add_to_bin(lds, bins.of(v), row.units(row.weigh(v))); });
+    // (the last bin: in a row of few heavy tokens, most)
+    uint32_t last_n = 0;
+    u64 last_units = 0;
+    row.each([&](uint32_t, float v) {
+        const uint32_t at = bins.of(v);
+        const u64 units = row.units(row.weigh(v));
+        if (at < kBins - 1u) {
+            add_to_bin(lds, at, units);
+        } else {
+            ++last_n;
+            last_units += units;
+        }
+    });
+    if (last_n) {
+        atomicAdd(&lds.count[kBins - 1u], last_n);
+        atomicAdd(&lds.mass[kBins - 1u], last_units);
+    }
     __syncthreads();
     Bin bin = find_bin(row, want, 0, [](u64) { return 0.0; }, lds);
     const uint32_t first = bin.at;
@@ -444,7 +460,7 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
     return cut_in_list(row, want, lds.list, bin.n, before, row.mass(mass_before), lds);
 }
 
-// A guess where the cut of a row lies, by a sample of it, the first eighth of every chunk: within three deviations, and where
+// A guess where the cut of a row lies, by a sample of it, an eighth of every chunk in kPieces places: within three deviations, and where
 // these hold too many tokens, within two.
 // (range: of logits, from the largest down, in which the cut is to be expected; total: not where the cut is by rank)
 struct Guess {
@@ -454,26 +470,35 @@ struct Guess {
 template <class E>
 __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, double total, uint32_t tokens, float range, RowLds& lds)
 {
-    constexpr uint32_t kPer = kChunk / 8, kVecs = kPer / E::kVec, kAhead = 40 / E::kVec;
+    constexpr uint32_t kPieces = 8, kPiece = kChunk / kPieces, kVecs = kPiece / 8u / E::kVec, kAhead = 40 / E::kVec;
     const Guess none = {0.0f, 0.0f, 0u, 0u};
     const Bins bins(row.max, range);
     clear_bins(lds);
     __syncthreads();
-    const uint32_t vecs = chunks_of(row.n) * kVecs;
+    uint32_t below = 0; // (in the last bin: in a row of few heavy tokens, most)
+    const uint32_t vecs = (row.n + kPiece - 1u) / kPiece * kVecs;
     for (uint32_t base = 0; base < vecs; base += kThreads * kAhead) {
         float v[kAhead][E::kVec];
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a) {
             const uint32_t i = base + a * kThreads + threadIdx.x;
-            load_tokens<E>(row.x, row.mask, i < vecs ? i / kVecs * kChunk + i % kVecs * E::kVec : row.n, row.n, v[a]);
+            load_tokens<E>(row.x, row.mask, i < vecs ? i / kVecs * kPiece + i % kVecs * E::kVec : row.n, row.n, v[a]);
         }
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll
             for (uint32_t k = 0; k < E::kVec; ++k)
-                if (v[a][k] > -INFINITY)
-                    atomicAdd(&lds.count[bins.of(v[a][k])], 1u);
+                if (v[a][k] > -INFINITY) {
+                    const uint32_t bin = bins.of(v[a][k]);
+                    if (bin < kBins - 1u)
+                        atomicAdd(&lds.count[bin], 1u);
+                    else
+                        ++below;
+                }
     }
+    below = __ockl_wfred_add_u32(below);
+    if (lane() == 0 && below)
+        atomicAdd(&lds.count[kBins - 1u], below);
     __syncthreads();
     // running sums of the bins, by rank of their tokens alone, by mass of what these weigh and of its squares too
     const uint32_t a = 2 * threadIdx.x;
@@ -524,6 +549,8 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     const float each = (float)tokens * __builtin_amdgcn_rcpf((float)samples);
     const double behind_goal = total - want.mass;
     double behind = sums - sum, var = squares_all - squares;
+    // (a small rank: few samples say little where tokens of like logits stand together)
+    const float margin = want.rank ? 512.0f : 0.0f;
     uint32_t n = upto, first[2] = {}, last[2] = {};
 #pragma unroll
     for (int k = 1; k >= 0; --k) {
@@ -534,7 +561,7 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
             const float z = tries ? 2.0f : 3.0f;
             if (far < -z * dev)
                 first[tries] = max(first[tries], a + (uint32_t)k + 1u);
-            if (far < z * dev)
+            if (far < z * dev || (far < z * dev + margin && a + (uint32_t)k + 1u < kBins - 1u))
                 last[tries] = max(last[tries], a + (uint32_t)k + 1u);
         }
         n -= c[k];
@@ -925,11 +952,12 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             lds.n = 0;
         if (plan.look) {
             double side = 0.0;
-            uint32_t above = 0;
+            uint32_t above = 0, n = 0;
             bool room = true;
             auto add = [&](const ChunkRec& one) {
                 side += one.sum;
                 above += one.count;
+                n += one.n_list;
                 room = room && one.n_list <= kLookList;
             };
 #pragma unroll
@@ -940,21 +968,28 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
                 add(recs[k]);
             side = __ockl_wfred_add_f64(side);
             above = __ockl_wfred_add_u32(above);
-            if (!__ballot(!room)) {
-                __syncthreads();
-                const uint32_t n = listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
-                if (n > 0 && n <= kList) {
-                    row.set_unit(plan.sums ? total : (double)kList);
-                    const float from = fminf(plan.high, row.max);
-                    list_bins = Bins(from, from - plan.low);
-                    bin_list(row, list_bins, n, lds);
-                    auto before = [&](u64 all) { return plan.from_above ? side : total - side - row.mass(all); };
-                    const Bin bin = find_bin(row, want, above, before, lds);
-                    // (is it there?)
-                    if (bin.n && !(above && want.reached(above, before(bin.all))))
-                        cut = cut_in_bin(row, want, list_bins, bin, n, above, before(bin.all), lds);
-                    listed_n = cut.n ? n : 0u;
+            n = __ockl_wfred_add_u32(n);
+            __syncthreads();
+            if (n > 0 && n <= kList) {
+                if (!__ballot(!room)) {
+                    (void)listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
+                } else { // (tokens that stand together: more in a chunk than its list holds)
+                    row.each([&](uint32_t id, float v) {
+                        if (v >= plan.low && v < plan.high)
+                            lds.list[atomicAdd(&lds.n, 1u)] = (uint64_t)order_key(v) << 32 | id;
+                    });
+                    __syncthreads();
                 }
+                row.set_unit(plan.sums ? total : (double)kList);
+                const float from = fminf(plan.high, row.max);
+                list_bins = Bins(from, from - plan.low);
+                bin_list(row, list_bins, n, lds);
+                auto before = [&](u64 all) { return plan.from_above ? side : total - side - row.mass(all); };
+                const Bin bin = find_bin(row, want, above, before, lds);
+                // (is it there?)
+                if (bin.n && !(above && want.reached(above, before(bin.all))))
+                    cut = cut_in_bin(row, want, list_bins, bin, n, above, before(bin.all), lds);
+                listed_n = cut.n ? n : 0u;
             }
         }
         if (cut.n == 0) {

@@ -28,7 +28,7 @@ struct RowKind {
         top_p = !greedy && p.top_p < 1.0f;
         top_k = greedy ? 0u : p.top_k;
         cut = min_p || top_p || top_k;
-        listed = top_k && top_k < n_vocab && (n_vocab <= kWholeRow || top_k <= min(kListTopK, kListShare * chunks_of(n_vocab)));
+        listed = top_k && top_k < n_vocab && top_k <= (n_vocab <= kWholeRow ? kListTopK : min(kListTopK, kListShare * chunks_of(n_vocab)));
         sums = !greedy && !listed;
         scale = weight_scale(p.temperature);
     }
