@@ -9,20 +9,17 @@ namespace mako {
 namespace step {
 namespace {
 
-// A lower bound of the n-th largest of the wave's values (of the least, if fewer lanes have a token; one has), to 16 bits of
-// their order.
-__device__ __forceinline__ float nth_largest(float v, uint32_t n)
+// Bits kHigh to kLow of the n-th largest of the wave's keys, behind those found before (n lanes have a key).
+template <int kHigh, int kLow>
+__device__ __forceinline__ uint32_t nth_largest(uint32_t key, uint32_t n, uint32_t found)
 {
-    n = min(n, (uint32_t)__popcll(__ballot(v > -INFINITY)));
-    const uint32_t key = ~order_key(v); // (rises with v)
-    uint32_t found = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = kHigh; bit >= kLow; --bit) {
         const uint32_t trial = found | 1u << bit;
         if ((uint32_t)__popcll(__ballot(key >= trial)) >= n)
             found = trial;
     }
-    return key_logit(~found);
+    return found;
 }
 
 __device__ __forceinline__ uint32_t lanes_before(unsigned long long lanes)
@@ -138,38 +135,45 @@ __global__ void __launch_bounds__(256, 6) scan_kernel(mako_cut_desc d, Scratch s
             rec.low = -__ockl_wfred_max_f32(-low);
         }
         if (kind.cut && d.n_vocab > kWholeRow) {
-            // The chunk's first tokens: those not below the n-th largest of the lanes' largest; above it, where these are too many
-            // (equal ones); of half as many lanes, where these are too many too.  A chunk of few tokens lists them all.
+            // The chunk's first tokens: those not below the n-th largest of the lanes' largest, to 16 bits of their order; where these
+            // are too many, to all bits, then those above it (equal ones), then of half as many lanes.  A chunk of few tokens lists
+            // them all.
             uint64_t* list = sc.lists + at * kChunkList;
-            auto take = [&](bool above) {
+            const bool all_listed = rec.count <= kChunkList;
+            const uint32_t key = ~order_key(mine); // (rises with the logit)
+            uint32_t n = min(kind.list_length(chunks), (uint32_t)__popcll(__ballot(mine > -INFINITY)));
+            uint32_t found = nth_largest<31, 16>(key, n, 0u);
+            rec.listed = all_listed ? -kFltMax : key_logit(~found);
+#pragma unroll 1
+            for (uint32_t tries = 0;; ++tries) {
                 rec.n_list = 0;
 #pragma unroll
                 for (int k = 0; k < kEach; ++k) {
-                    const bool in = above ? x[k] > rec.listed : x[k] >= rec.listed;
+                    const bool in = x[k] >= rec.listed;
                     const unsigned long long all = __ballot(in);
                     if (all) {
-                        const uint32_t n = (uint32_t)__popcll(all);
-                        if (rec.n_list + n <= kChunkList)
+                        const uint32_t more = (uint32_t)__popcll(all);
+                        if (rec.n_list + more <= kChunkList)
                             c.put(list, k, in, all, rec.n_list);
-                        rec.n_list += n;
+                        rec.n_list += more;
                     }
                 }
-            };
-            rec.listed = INFINITY;
-            for (uint32_t n = rec.count <= kChunkList ? 64u : kind.list_length(chunks); n; n /= 2u) {
-                rec.listed = rec.count <= kChunkList ? -kFltMax : nth_largest(mine, n);
-                take(false);
                 if (rec.n_list <= kChunkList)
                     break;
-                take(true);
-                if (rec.n_list <= kChunkList) {
+                if (tries % 2u == 0) {
+                    n = tries ? n / 2u : n;
+                    if (n == 0) {
+                        rec.listed = INFINITY;
+                        rec.n_list = 0;
+                        break;
+                    }
+                    found = nth_largest<15, 0>(key, n, tries ? nth_largest<31, 16>(key, n, 0u) : found);
+                    rec.listed = key_logit(~found);
+                } else {
                     rec.listed = key_logit(order_key(rec.listed + 0.0f) - 1u); // (all of the next larger number and above)
-                    break;
                 }
-                rec.listed = INFINITY;
-                rec.n_list = 0;
             }
-            if (rec.count <= kChunkList)
+            if (all_listed)
                 rec.listed = -INFINITY;
         } else {
 #pragma unroll
