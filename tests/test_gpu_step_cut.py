@@ -10,8 +10,11 @@ pytestmark = pytest.mark.gpu
 
 # A weight is exp(t) with t = (x - max) / T, of rounded numbers: t has an error of 3 half steps (the difference, the reciprocal
 # of T, the product), which is 3 |t| 2^-53 of the weight, 3e-14 at t = -90; weights below that are nothing beside the first.
-# exp itself is within 2^-49 on both sides.  What a cut leaves is added up in whole units of 2^-60 of the total: at most 2^20
-# of them are lost, 2^-40 = 9.1e-13 of it.  The sums' own roundings (20 levels, 2^-53 each) do not show beside that.
+# The kernels' 2^t is within 2.7e-14, exp here within 2^-52.  What a cut leaves is added up in whole units, each token's weight
+# off by half of one.  Rows whose weights are summed up beforehand: a unit is at most 2^-62 of that sum, and what a top_p leaves
+# at least a twentieth of it here: 2^18 2^-63 / 0.05 = 5.7e-13 of it (with top_p of 0.5 and more, 2^20 tokens 2.3e-13).  Rows of
+# a top_k of up to 2500: a unit is at most 2^-50, and a total at least 1: 2500 2^-51 = 1.11e-12.  The sums' own roundings (20
+# levels, 2^-53 each) are 2.2e-15.  All together 1.17e-12.
 TOTAL = 1.2e-12
 # a probability is rounded to fp32: half a step, 2^-24, and below the normal range half of 2^-149
 PROB, PROB_LEAST = 2.0**-24 + 1e-11, 2.0**-150
@@ -186,3 +189,52 @@ def test_lowest_cut_is_a_finite_number(ctx):
     x = np.full((1, 3000), -FLT_MAX, np.float32)
     got = check(ctx, x, api.make_params(1, top_k=1234))
     assert got[0]["cut_token"] == 1233 and got[0]["cut_logit"] == -FLT_MAX
+
+
+@pytest.mark.parametrize("vocab", [6143, 6144, 6145, 6200])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_that_are_held_whole_and_the_next_larger(ctx, vocab, dtype):
+    rng = np.random.default_rng(vocab)
+    rows = 2 * len(KINDS)
+    p = all_kinds(rows)
+    p["top_k"][1], p["temperature"][1] = vocab - 1, 2.0
+    p["top_k"][11], p["temperature"][11], p["top_p"][11] = 5000, 2.0, 0.99
+    x = rng.normal(0, 3, (rows, vocab))
+    x[::2] *= 0.01
+    check(ctx, x, p, dtype)
+
+
+def odd_rows(kind, rows, vocab, rng):
+    x = rng.normal(0, 3, (rows, vocab)).astype(np.float32)
+    if kind == "falling":
+        x = -np.sort(-x, axis=1)
+    elif kind == "rising":
+        x = np.sort(x, axis=1)
+    elif kind == "outlier":
+        x[:, 77] = 1000.0
+    elif kind == "heavy":
+        x = (x / rng.normal(0, 1, (rows, vocab))).astype(np.float32)
+    elif kind == "two":
+        x[:, rng.random(vocab) < 0.5] -= 500.0
+    elif kind == "narrow":
+        x = (20.0 + 0.01 * x).astype(np.float32)
+    elif kind == "together":
+        x[:, 5000:9000] += 12.0
+    elif kind == "ends":
+        x[:, -1] = 30.0
+        x[:, 0] = 30.0
+    return x
+
+
+@pytest.mark.parametrize("kind", ["falling", "rising", "outlier", "heavy", "two", "narrow", "together", "ends"])
+def test_rows_that_no_sample_and_no_list_fits(ctx, kind):
+    """Where samples mislead and lists overflow: tokens in order or together, one far above, two crowds far apart."""
+    rng = np.random.default_rng(len(kind) * 100 + ord(kind[0]))
+    ways = [dict(top_p=0.9), dict(top_p=0.5), dict(temperature=50.0, top_p=0.9), dict(top_k=40), dict(top_k=1000, top_p=0.9), dict(top_k=1250), dict(top_k=1300),
+            dict(top_k=2500, top_p=0.99), dict(top_k=2501), dict(top_k=3500), dict(top_k=20000, top_p=0.9), dict(top_k=70000), dict(min_p=0.05),
+            dict(min_p=1e-4, top_p=0.95), dict(min_p=1e-30), dict(temperature=0.05, top_p=0.99)]
+    p = api.make_params(len(ways))
+    for r, w in enumerate(ways):
+        for f, v in w.items():
+            p[f][r] = v
+    check(ctx, odd_rows(kind, len(ways), 80021, rng), p)
