@@ -39,8 +39,8 @@ extern "C" {
 typedef struct mako_step_ctx mako_step_ctx;
 
 /* Creates a context on HIP device `device` for rows (requests) of up to max_rows and vocabularies of up to max_vocab
- * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB); its scratch memory (2.5 bytes for every logit of the
- * largest batch, and 220 a row) is allocated here. */
+ * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB); its scratch memory (some 2.5 bytes for every logit of
+ * the largest batch, and 160 a row) is allocated here. */
 #define MAKO_STEP_MAX_ROWS 65535
 #define MAKO_STEP_MAX_VOCAB 1048576
 int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_t max_vocab);

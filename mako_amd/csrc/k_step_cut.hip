@@ -7,6 +7,19 @@
 //   look_kernel   (k_step_scan.hip) the rows that have a plan: the tokens there, and what lies above them, or below
 //   wide_kernel   these rows, a workgroup each: the cut among those tokens, or, should it not be there, by dividing the row
 //   probs_kernel  where asked for: the rows as probabilities
+//
+// The mathematics: with the weights w = exp((x - max) / T), a row's cut is the place in the order of falling logits behind a rank
+// (min_p and top_k come down to one) or behind the least number of tokens that weigh top_p of all.  No row is sorted: the pass
+// over it leaves some 10 to 71 of every 2048 tokens, among which a narrow cut lies; a wide one is guessed by a sample of an
+// eighth of the row, and a second pass collects the tokens around it and adds up those above.  Among at most 6144 tokens, in LDS,
+// 1024 bins of logits say which bin holds it, and the bin's tokens are counted against each other.  Weights are 64-bit floats, and
+// where they are added up in an order that chance makes (bins, atomics) whole numbers of a unit, so that results do not vary.
+//
+// What bounds them: 64 rows of 129280 fp32 logits (33.1 MB), some cut beyond their lists, take 44 us: scan 12.4 (2.7 TB/s), row 12.9,
+// look 7.9, wide 10; one row of 151552 34: 5.6, 12.4, 7.2, 8.7; 256 of them, half of them flat, 95: 43 (3.6 TB/s, vector
+// instructions 70 % of the time), 15, 24 (6.4 TB/s, from the Infinity Cache) and 12.  row_kernel and wide_kernel are chains of some
+// fifteen trips to memory, LDS and barriers with one workgroup's latency in each, their code read from memory as they go (a pass
+// fewer through the list, with the exponentials in more places, took 1 us longer).
 #include "step_common.h"
 #include "step_cut.h"
 #include "step_launch.h"
@@ -15,11 +28,11 @@ namespace mako {
 namespace step {
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kThreads = 512, kWaves = kThreads / 64; // two workgroups to a CU, by LDS
 constexpr uint32_t kBins = 1024;  // two to a thread
 constexpr uint32_t kList = kWholeRow; // tokens that are held in LDS
 constexpr uint32_t kSmall = 1024; // ... of a bin
-constexpr uint32_t kCrowd = 256;  // ... that are counted against each other
+constexpr uint32_t kCrowd = 256;  // ... that are counted against each other; more are sorted
 static_assert(kBins == 2 * kThreads, "two bins to a thread");
 
 typedef unsigned long long u64;
@@ -460,8 +473,10 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
     return cut_in_list(row, want, lds.list, bin.n, before, row.mass(mass_before), lds);
 }
 
-// A guess where the cut of a row lies, by a sample of it, an eighth of every chunk in kPieces places: within three deviations, and where
-// these hold too many tokens, within two.
+// A guess where the cut of a row lies, by a sample of it, an eighth of every chunk in kPieces places (128 bytes of fp32 each): within
+// three deviations, and where these hold too many tokens, within two.  (7 of row_kernel's 12.4 us on one row of 151552, 4 of them
+// the sample; a sixteenth took as long, with longer lists for wide_kernel.  In one place the times are the same, but rows whose
+// tokens stand in order are guessed wrongly and divided: 290 us instead of 80.)
 // (range: of logits, from the largest down, in which the cut is to be expected; total: not where the cut is by rank)
 struct Guess {
     float low, high;
@@ -1069,7 +1084,7 @@ __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
     }
 }
 
-constexpr uint32_t kWideWorkgroups = 512; // (two to a CU: what fits)
+constexpr uint32_t kWideWorkgroups = 512; // (two to a CU: what fits; 512 wide rows of 32000 take 75 us in all, with 256 workgroups 82)
 template <class E>
 void cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
