@@ -17,7 +17,7 @@
 //
 // What bounds them: 64 rows of 129280 fp32 logits (33.1 MB), some cut beyond their lists, take 44 us: scan 12.4 (2.7 TB/s), row 12.9,
 // look 7.9, wide 10; one row of 151552 34: 5.6, 12.4, 7.2, 8.7; 256 of them, half of them flat, 95: 43 (3.6 TB/s, vector
-// instructions 70 % of the time), 15, 24 (6.4 TB/s, from the Infinity Cache) and 12.  row_kernel and wide_kernel are chains of some
+// instructions 78 % of the time), 15, 24 (6.4 TB/s, from the Infinity Cache) and 12.  row_kernel and wide_kernel are chains of some
 // fifteen trips to memory, LDS and barriers with one workgroup's latency in each, their code read from memory as they go (a pass
 // fewer through the list, with the exponentials in more places, took 1 us longer).
 #include "step_common.h"
@@ -34,6 +34,7 @@ constexpr uint32_t kList = kWholeRow; // tokens that are held in LDS
 constexpr uint32_t kSmall = 1024; // ... of a bin
 constexpr uint32_t kCrowd = 256;  // ... that are counted against each other; more are sorted
 static_assert(kBins == 2 * kThreads, "two bins to a thread");
+constexpr int kTries = 3; // how wide a guess may be
 
 typedef unsigned long long u64;
 
@@ -48,7 +49,7 @@ struct RowLds {
     Share<kWaves> share;
     uint32_t counts[kWaves];
     double squares[kWaves];
-    uint32_t first_bin[2], last_bin[2], n_before[2], n_upto[2];
+    uint32_t first_bin[kTries], last_bin[kTries], n_before[kTries], n_upto[kTries];
     uint32_t n, at, before, id, first;
     u64 mass_before;
     double m;
@@ -474,7 +475,7 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
 }
 
 // A guess where the cut of a row lies, by a sample of it, an eighth of every chunk in kPieces places (128 bytes of fp32 each): within
-// three deviations, and where these hold too many tokens, within two.  (7 of row_kernel's 12.4 us on one row of 151552, 4 of them
+// four deviations, and where these hold too many tokens, within three, or two and a half.  (7 of row_kernel's 12.4 us on one row of 151552, 4 of them
 // the sample; a sixteenth took as long, with longer lists for wide_kernel.  In one place the times are the same, but rows whose
 // tokens stand in order are guessed wrongly and divided: 290 us instead of 80.)
 // (range: of logits, from the largest down, in which the cut is to be expected; total: not where the cut is by rank)
@@ -538,7 +539,8 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
         lds.squares[wave()] = squares;
     }
     if (threadIdx.x == 0)
-        lds.first_bin[0] = lds.last_bin[0] = lds.first_bin[1] = lds.last_bin[1] = 0;
+        for (int tries = 0; tries < kTries; ++tries)
+            lds.first_bin[tries] = lds.last_bin[tries] = 0;
     __syncthreads();
     uint32_t samples = 0, n_all = 0;
     double sums = 0.0, sum_all = 0.0, squares_before = 0.0, squares_all = 0.0;
@@ -566,14 +568,14 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     double behind = sums - sum, var = squares_all - squares;
     // (a small rank: few samples say little where tokens of like logits stand together)
     const float margin = want.rank ? 512.0f : 0.0f;
-    uint32_t n = upto, first[2] = {}, last[2] = {};
+    uint32_t n = upto, first[kTries] = {}, last[kTries] = {};
 #pragma unroll
     for (int k = 1; k >= 0; --k) {
         const float far = want.rank ? (float)n * each - (float)want.rank : (float)(behind_goal - behind * (double)each);
         const float dev = each * __builtin_amdgcn_sqrtf(want.rank ? (float)n + 1.0f : (float)fmax(var, 0.0));
 #pragma unroll
-        for (int tries = 0; tries < 2; ++tries) {
-            const float z = tries ? 2.0f : 3.0f;
+        for (int tries = 0; tries < kTries; ++tries) {
+            const float z = tries == 0 ? 4.0f : (tries == 1 ? 3.0f : 2.5f);
             if (far < -z * dev)
                 first[tries] = max(first[tries], a + (uint32_t)k + 1u);
             if (far < z * dev || (far < z * dev + margin && a + (uint32_t)k + 1u < kBins - 1u))
@@ -584,7 +586,7 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
         var += w[k] * w[k] * c[k];
     }
 #pragma unroll
-    for (int tries = 0; tries < 2; ++tries) {
+    for (int tries = 0; tries < kTries; ++tries) {
         first[tries] = __ockl_wfred_max_u32(first[tries]);
         last[tries] = __ockl_wfred_max_u32(last[tries]);
         if (lane() == 0) {
@@ -594,7 +596,7 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     }
     __syncthreads();
 #pragma unroll
-    for (int tries = 0; tries < 2; ++tries) {
+    for (int tries = 0; tries < kTries; ++tries) {
         n = upto - c[0] - c[1];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -606,7 +608,7 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
         }
     }
     __syncthreads();
-    for (int tries = 0; tries < 2; ++tries) {
+    for (int tries = 0; tries < kTries; ++tries) {
         const uint32_t first_bin = lds.first_bin[tries], last_bin = lds.last_bin[tries];
         if (last_bin >= kBins - 1u) // (the last bin has no lower end)
             return none;
@@ -961,10 +963,12 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
         double total = plan.total;
         Bins list_bins(row.max, 1.0f);
         uint32_t listed_n = 0; // tokens in lds.list, where the cut is
+        float low = plan.low, high = plan.high;
         __syncthreads();
         clear_bins(lds);
         if (threadIdx.x == 0)
             lds.n = 0;
+        row.set_unit(plan.sums ? total : (double)kList);
         if (plan.look) {
             double side = 0.0;
             uint32_t above = 0, n = 0;
@@ -984,27 +988,61 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
             side = __ockl_wfred_add_f64(side);
             above = __ockl_wfred_add_u32(above);
             n = __ockl_wfred_add_u32(n);
+            room = !__ballot(!room) && n <= kList;
             __syncthreads();
-            if (n > 0 && n <= kList) {
-                if (!__ballot(!room)) {
-                    (void)listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
-                } else { // (tokens that stand together: more in a chunk than its list holds)
-                    row.each([&](uint32_t id, float v) {
-                        if (v >= plan.low && v < plan.high)
-                            lds.list[atomicAdd(&lds.n, 1u)] = (uint64_t)order_key(v) << 32 | id;
-                    });
-                    __syncthreads();
-                }
-                row.set_unit(plan.sums ? total : (double)kList);
-                const float from = fminf(plan.high, row.max);
-                list_bins = Bins(from, from - plan.low);
+            if (room) {
+                (void)listed.gather(c, recs, lists, chunks, -INFINITY, INFINITY, lds);
+                const float from = fminf(high, row.max);
+                list_bins = Bins(from, from - low);
                 bin_list(row, list_bins, n, lds);
                 auto before = [&](u64 all) { return plan.from_above ? side : total - side - row.mass(all); };
                 const Bin bin = find_bin(row, want, above, before, lds);
-                // (is it there?)
-                if (bin.n && !(above && want.reached(above, before(bin.all))))
+                if (above && want.reached(above, before(bin.all))) {
+                    const float width = from - low;
+                    low = high;
+                    high += 2.0f * width;
+                } else if (bin.n) {
                     cut = cut_in_bin(row, want, list_bins, bin, n, above, before(bin.all), lds);
-                listed_n = cut.n ? n : 0u;
+                    listed_n = n;
+                } else {
+                    high = low;
+                    low -= 2.0f * (from - low);
+                }
+            }
+            if (cut.n == 0) {
+                // Too many tokens for a chunk's list (they stand together), or the cut is beside them: in a pass over the row by this
+                // workgroup alone, there.  (One row in some thousands: 40 us, a division of a row of 129280 takes 100 and more.)
+                u64 units = 0, all;
+                above = 0;
+                clear_bins(lds);
+                if (threadIdx.x == 0)
+                    lds.n = 0;
+                __syncthreads();
+                row.each([&](uint32_t id, float v) {
+                    if (v >= high) {
+                        ++above;
+                        units += row.units(row.weigh(v));
+                    } else if (v >= low) {
+                        const uint32_t at = atomicAdd(&lds.n, 1u);
+                        if (at < kList)
+                            lds.list[at] = (uint64_t)order_key(v) << 32 | id;
+                    }
+                });
+                above = all_sum<kWaves>(above, lds.share);
+                (void)sum_before<kWaves>(units, all, lds.share);
+                n = lds.n;
+                __syncthreads();
+                if (n <= kList) {
+                    const double weight_above = row.mass(all);
+                    const float from = fminf(high, row.max);
+                    list_bins = Bins(from, from - low);
+                    bin_list(row, list_bins, n, lds);
+                    const Bin bin = find_bin(row, want, above, [&](u64) { return weight_above; }, lds);
+                    if (bin.n && !(above && want.reached(above, weight_above))) {
+                        cut = cut_in_bin(row, want, list_bins, bin, n, above, weight_above, lds);
+                        listed_n = n;
+                    }
+                }
             }
         }
         if (cut.n == 0) {
@@ -1015,7 +1053,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
         if (plan.rank && plan.top_p < 1.0f) {
             want = Want{0, (double)plan.top_p * cut.mass};
             cut.n = 0;
-            if (listed_n && plan.high == INFINITY)
+            if (listed_n && high == INFINITY)
                 cut = cut_in_bins(row, want, list_bins, listed_n, lds);
             if (cut.n == 0) {
                 if (!plan.sums && total == 0.0)

@@ -4,10 +4,11 @@
 //
 // A chunk is 32 logits a lane, in registers from the one load to the last list entry: the largest, the number, the sum of the
 // weights relative to the chunk's own largest (rescaled where the chunks come together) and the list need no second load and no
-// barrier.  Bound by vector instructions and memory alike: 512 rows of 129280 bf16 logits (132 MB) 41.6 us, 538 instructions a
-// chunk where a top_k needs no sums, 256 rows of 151552 fp32 logits (155 MB) 43 us, 919 with sums, 20 a logit of them for its
-// weight (arithmetic in 64 bits runs at the full rate here).  Chunks of 1024 logits, with as many reductions and searches for half
-// the work, took 60 us for both.
+// barrier.  Bound by vector instructions (80 % of the time), with memory close behind: 512 rows of 129280 bf16 logits (132 MB) 41
+// us, some 540 instructions a chunk, most of them without sums, 256 rows of 151552 fp32 logits (155 MB) 43 us, 914 with sums, 20 a
+// logit of them for its weight (arithmetic in 64 bits runs at the full rate here).  Chunks of 1024 logits, with as many reductions
+// and searches for half the work, took 60 us for both; largest and smallest by instructions that take three logits spill fp32's
+// registers (69 us) and gain bf16 nothing.
 #include "step_common.h"
 #include "step_cut.h"
 #include "step_launch.h"
