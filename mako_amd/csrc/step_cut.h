@@ -8,7 +8,7 @@ namespace mako {
 namespace step {
 
 // Rows of no more logits than this are held whole where they are cut, and have no lists: 64 rows of 6144 cut to a top_p take 19 us, of
-// 6145 with lists 35, to a top_k of 50 14 and 16.  (The more are held, the fewer workgroups a CU has: 49 of 160 KB of LDS here.)
+// 6145 with lists 36, to a top_k of 50 14 and 16.  (The more are held, the fewer workgroups a CU has: 49 of 160 KB of LDS here.)
 constexpr uint32_t kWholeRow = 6144;
 
 // Largest top_k that is looked for in the chunks' lists, of a row and of a chunk's share of it.  (64 rows of 129280, 64 chunks: top_k
