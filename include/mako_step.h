@@ -145,7 +145,8 @@ int mako_step_verify_drafts(mako_step_ctx* ctx, const mako_verify_desc* desc, vo
  *      max_tokens; the others get status MAKO_BLOCKS_TOKENS and no blocks (step 3 had counted what they ask for).
  * A request that is refused keeps its blocks and has no tokens in the step.  One that has ended is passed with lengths of 0: it
  * gives all its blocks back.  One with a length below 0 is not there: it keeps its blocks and has no tokens.
- * Entries of a table beyond what a request holds are never read, and are left as they are unless blocks are put there. */
+ * Entries of a table beyond what a request holds are never read, and are left as they are unless blocks are put there.  Blocks
+ * are not counted: one that stands in two tables is given back by each. */
 #define MAKO_BLOCKS_OK 0
 #define MAKO_BLOCKS_SHORT 1
 #define MAKO_BLOCKS_WIDE 2

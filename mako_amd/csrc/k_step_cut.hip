@@ -96,9 +96,7 @@ struct Row {
         constexpr uint32_t kStep = kThreads * E::kVec, kAhead = 16 / E::kVec;
         for (uint32_t base = 0; base < n; base += kStep * kAhead) {
             float v[kAhead][E::kVec];
-#pragma unroll
-            for (uint32_t a = 0; a < kAhead; ++a)
-                load_tokens<E>(x, mask, base + a * kStep + threadIdx.x * E::kVec, n, v[a]);
+            load_tokens<E>(x, mask, [&](uint32_t a) { return base + a * kStep + threadIdx.x * E::kVec; }, n, v);
 #pragma unroll
             for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll
@@ -441,8 +439,9 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
         uint32_t seen = 0;
         constexpr uint32_t kStep = kThreads * E::kVec;
         for (uint32_t base = 0; base < row.n && seen < rank; base += kStep) {
-            float x[E::kVec];
-            load_tokens<E>(row.x, row.mask, base + threadIdx.x * E::kVec, row.n, x);
+            float v1[1][E::kVec];
+            load_tokens<E>(row.x, row.mask, [&](uint32_t) { return base + threadIdx.x * E::kVec; }, row.n, v1);
+            const float(&x)[E::kVec] = v1[0];
             uint32_t mine = 0;
 #pragma unroll
             for (uint32_t k = 0; k < E::kVec; ++k)
@@ -495,11 +494,11 @@ __device__ __forceinline__ Guess guess(const Row<E>& row, const Want& want, doub
     const uint32_t vecs = (row.n + kPiece - 1u) / kPiece * kVecs;
     for (uint32_t base = 0; base < vecs; base += kThreads * kAhead) {
         float v[kAhead][E::kVec];
-#pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
+        auto at = [&](uint32_t a) {
             const uint32_t i = base + a * kThreads + threadIdx.x;
-            load_tokens<E>(row.x, row.mask, i < vecs ? i / kVecs * kPiece + i % kVecs * E::kVec : row.n, row.n, v[a]);
-        }
+            return i < vecs ? i / kVecs * kPiece + i % kVecs * E::kVec : row.n;
+        };
+        load_tokens<E>(row.x, row.mask, at, row.n, v);
 #pragma unroll
         for (uint32_t a = 0; a < kAhead; ++a)
 #pragma unroll

@@ -113,16 +113,32 @@ __device__ __forceinline__ float token_logit(float x, bool allowed)
     return allowed && x > -INFINITY ? fminf(x, kFltMax) + 0.0f : -INFINITY;
 }
 
-template <class E>
-__device__ __forceinline__ void load_tokens(const void* row, const uint32_t* mask, uint32_t i, uint32_t n, float* x)
+// N vectors of a row's logits as token_logit() gives them, the a-th from token at(a) on (a multiple of kVec: its mask bits lie in one
+// word), all asked for before any is looked at.
+template <class E, uint32_t N, class F>
+__device__ __forceinline__ void load_tokens(const void* row, const uint32_t* mask, F at, uint32_t n, float (&x)[N][E::kVec])
 {
-    load_vec<E>(row, i, n, x);
-    uint32_t bits = 0xffffffffu;
-    if (mask) // (i is a multiple of kVec: the vector's bits lie in one word)
-        bits = i < n ? mask[i >> 5] >> (i & 31u) : 0u;
 #pragma unroll
-    for (uint32_t k = 0; k < E::kVec; ++k)
-        x[k] = token_logit(x[k], (bits >> k) & 1u);
+    for (uint32_t a = 0; a < N; ++a)
+        load_vec<E>(row, at(a), n, x[a]);
+    if (mask) {
+        uint32_t bits[N];
+#pragma unroll
+        for (uint32_t a = 0; a < N; ++a)
+            bits[a] = at(a) < n ? mask[at(a) >> 5] >> (at(a) & 31u) : 0u;
+#pragma unroll
+        for (uint32_t a = 0; a < N; ++a)
+#pragma unroll
+            for (uint32_t k = 0; k < E::kVec; ++k) {
+                const uint32_t keep = (uint32_t)((int32_t)(bits[a] << (31u - k)) >> 31);
+                x[a][k] = __uint_as_float((__float_as_uint(x[a][k]) & keep) | (0xff800000u & ~keep));
+            }
+    }
+#pragma unroll
+    for (uint32_t a = 0; a < N; ++a)
+#pragma unroll
+        for (uint32_t k = 0; k < E::kVec; ++k)
+            x[a][k] = fminf(fmaxf(x[a][k], -INFINITY), kFltMax) + 0.0f; // (of a NaN and a number, the number)
 }
 
 // Rising keys are falling logits.
