@@ -7,8 +7,8 @@
 // Of a request's rows only one is read whole, the one behind the last accepted draft, and of the drafter's the one beside it: which
 // these are follows from one logit of each row, which every workgroup looks up for itself (a launch of its own would cost more).
 // What is left, max(0, p - q), is needed as a sum before a token can be drawn by it: the parts' sums first, then one part again.
-// 64 requests over 129280 bf16 logits of each kind (33 MB) take 15.1 and 5.5 us, one over 151552 fp32 logits 5.5 and 4.4, 32 with
-// looked-up drafts under masks 7.1 and 4.9, 256 over 32000 probabilities (66 MB) 12.4 and 4.8: large ones are bound by
+// 64 requests over 129280 bf16 logits of each kind (33 MB) take 14.1 and 5.0 us, one over 151552 fp32 logits 5.6 and 4.4, 32 with
+// looked-up drafts under masks 7.4 and 5.1, 256 over 32000 probabilities (66 MB) 11.7 and 4.5: large ones are bound by
 // memory and the weights' arithmetic (two weights of 20 instructions a token), small ones by five trips to memory in a row, draw_kernel
 // always.
 #include "step_common.h"
@@ -100,26 +100,21 @@ struct Left {
         minus_q = false;
         without = kNoToken;
     }
-    // p's tokens of a part, four to a thread, and q's
-    __device__ __forceinline__ void load(uint32_t at, float* v, float* w) const
+    // p's tokens of a part, four to a thread; whether any of the wave's may have something left; and q's
+    __device__ __forceinline__ void load_p(uint32_t at, float* v) const { p.load(at * kPart + threadIdx.x * 4u, (at + 1u) * kPart <= p.n, v); }
+    __device__ __forceinline__ bool any(const float* v) const
     {
-        const bool whole = (at + 1u) * kPart <= p.n;
-        p.load(at * kPart + threadIdx.x * 4u, whole, v);
+        return __ballot(p.may_keep(v[0]) || p.may_keep(v[1]) || p.may_keep(v[2]) || p.may_keep(v[3])) != 0;
+    }
+    __device__ __forceinline__ void load_q(uint32_t at, float* w) const
+    {
         if (minus_q)
-            q.load(at * kPart + threadIdx.x * 4u, whole, w);
+            q.load(at * kPart + threadIdx.x * 4u, (at + 1u) * kPart <= p.n, w);
     }
     // and what they have left
     __device__ __forceinline__ void four(uint32_t at, const float* v, const float* w, double* r) const
     {
         const uint32_t i = at * kPart + threadIdx.x * 4u;
-        bool any = false;
-#pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k) {
-            any = any || p.may_keep(v[k]);
-            r[k] = 0.0;
-        }
-        if (!__ballot(any))
-            return;
         p.four(i, v, r);
         if (minus_q) {
             double s[4];
@@ -136,8 +131,12 @@ struct Left {
     __device__ __forceinline__ void part(uint32_t at, double* r) const
     {
         float v[4], w[4];
-        load(at, v, w);
-        four(at, v, w, r);
+        load_p(at, v);
+        r[0] = r[1] = r[2] = r[3] = 0.0;
+        if (any(v)) {
+            load_q(at, w);
+            four(at, v, w, r);
+        }
     }
 };
 
@@ -229,7 +228,7 @@ __device__ __forceinline__ Left<E, Q> left_of(const mako_verify_desc& d, uint32_
 }
 
 template <class E, class Q>
-__global__ void __launch_bounds__(kThreads, 6) left_kernel(mako_verify_desc d, Scratch sc, uint32_t each)
+__global__ void __launch_bounds__(kThreads, 8) left_kernel(mako_verify_desc d, Scratch sc, uint32_t each)
 {
     __shared__ double sums[kMostParts][kWaves];
     __shared__ Words<Stop> shared;
@@ -252,23 +251,37 @@ __global__ void __launch_bounds__(kThreads, 6) left_kernel(mako_verify_desc d, S
     for (uint32_t k = 0; k < sizeof(Stop) / 4u; ++k)
         known.words[k] = __builtin_amdgcn_readfirstlane(shared.words[k]);
     const Left<E, Q> left = left_of<E, Q>(d, b, known.value);
-    // (a part's loads are on their way while the part before it is added up)
-    float v[4], w[4];
-    left.load(first, v, w);
+    // (p's tokens are on their way two parts ahead, q's one, and only where a wave's 256 tokens of p have something left: in a row cut
+    // to a narrow nucleus most have not)
+    float v[4], w[4], next_v[4];
+    left.load_p(first, v);
+    if (n > 1u)
+        left.load_p(first + 1u, next_v);
+    bool here = left.any(v);
+    if (here)
+        left.load_q(first, w);
 #pragma unroll 1
     for (uint32_t j = 0; j < n; ++j) {
-        float next_v[4], next_w[4];
-        if (j + 1u < n)
-            left.load(first + j + 1u, next_v, next_w);
-        double r[4];
-        left.four(first + j, v, w, r);
-        const double sum = __ockl_wfred_add_f64(r[0] + r[1] + r[2] + r[3]);
+        float next_w[4], after_v[4];
+        const bool next = j + 1u < n && left.any(next_v);
+        if (next)
+            left.load_q(first + j + 1u, next_w);
+        if (j + 2u < n)
+            left.load_p(first + j + 2u, after_v);
+        double sum = 0.0;
+        if (here) {
+            double r[4];
+            left.four(first + j, v, w, r);
+            sum = __ockl_wfred_add_f64(r[0] + r[1] + r[2] + r[3]);
+        }
         if (lane() == 0)
             sums[j][wave()] = sum;
+        here = next;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             v[k] = next_v[k];
             w[k] = next_w[k];
+            next_v[k] = after_v[k];
         }
     }
     __syncthreads();
@@ -378,8 +391,8 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
     }
 }
 
-// (more workgroups find the place anew, fewer wait longer for their loads: the three larger calls above take 15.5, 8.0 and 14.7 us with
-// 2048, 21.1, 7.9 and 16.6 with 1024, 17.0, 12.3 and 15.2 with 4096)
+// (as many as run at a time.  More find the place anew, fewer wait longer for their loads: with 1024 the three larger calls above took
+// 21.1, 7.9 and 16.6 us when with 2048 they took 15.5, 8.0 and 14.7, with 4096 17.0, 12.3 and 15.2)
 constexpr uint32_t kWorkgroups = 2048;
 template <class E, class Q>
 void verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
