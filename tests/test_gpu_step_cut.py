@@ -238,3 +238,31 @@ def test_rows_that_no_sample_and_no_list_fits(ctx, kind):
         for f, v in w.items():
             p[f][r] = v
     check(ctx, odd_rows(kind, len(ways), 80021, rng), p)
+
+
+def test_more_rows_than_workgroups():
+    """More rows with a cut beyond their lists than the kernels for these have workgroups: 50 rows over and over."""
+    rng = np.random.default_rng(31)
+    p = api.make_params(50, top_p=0.8)
+    p["top_k"][::5], p["top_p"][::5] = 2000, 1.0
+    p["temperature"][1::5] = 0.0
+    p["top_p"][2::5], p["min_p"][2::5] = 1.0, 0.2
+    x = rng.normal(0, 0.5, (50, 8192)).astype(np.float32)
+    c = step.StepContext(max_rows=5000, max_vocab=8192)
+    few = check(c, x, p, "float16")
+    many, _ = cut_rows(c, np.tile(x, (100, 1)), np.tile(p, 100), "float16")
+    assert many.tobytes() == few.tobytes() * 100
+    c.close()
+
+
+def test_as_many_rows_as_there_may_be():
+    rng = np.random.default_rng(32)
+    x = rng.normal(0, 3, (51, 40)).astype(np.float32)
+    p = all_kinds(51)
+    c = step.StepContext(max_rows=step.MAX_ROWS, max_vocab=40)
+    few = check(c, x, p, probs=True)
+    _, few_probs = cut_rows(c, x, p, probs=True)
+    many, many_probs = cut_rows(c, np.tile(x, (1285, 1)), np.tile(p, 1285), probs=True)
+    assert len(many) == step.MAX_ROWS
+    assert many.tobytes() == few.tobytes() * 1285 and many_probs.tobytes() == few_probs.tobytes() * 1285
+    c.close()

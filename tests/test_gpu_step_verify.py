@@ -247,3 +247,19 @@ def test_tokens_are_distributed_as_the_targets(ctx):
     rate = out["accepted"].download().mean()
     want = np.minimum(p, q).sum()
     assert abs(rate - want) <= 5 * np.sqrt(want * (1 - want) / n)
+
+
+def test_as_many_requests_as_there_may_be():
+    rng = np.random.default_rng(33)
+    few, times = 257, step.MAX_ROWS // 257
+    c = step.StepContext(max_rows=step.MAX_ROWS, max_vocab=30)
+    case = make(rng, few, 2, 30, "probs")
+    got = run(c, case)
+    b = Buffers()
+    many = {f: np.tile(a, (times,) + (1,) * (a.ndim - 1)) if isinstance(a, np.ndarray) else a for f, a in case.items()}
+    desc, out = verify_desc(b, **many)
+    c.verify_drafts(desc)
+    hip.synchronize()
+    for f, a in out.items():
+        assert np.array_equal(a.download(), np.tile(got[f], (times,) + (1,) * (got[f].ndim - 1))), f
+    c.close()
