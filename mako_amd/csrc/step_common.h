@@ -252,19 +252,6 @@ __device__ __forceinline__ uint32_t all_min(uint32_t v, Share<W>& s)
     __syncthreads();
     return t;
 }
-template <int W>
-__device__ __forceinline__ float all_max(float v, Share<W>& s)
-{
-    v = __ockl_wfred_max_f32(v);
-    if (lane() == 0)
-        s.d[wave()] = (double)v;
-    __syncthreads();
-    float t = -INFINITY;
-    for (int w = 0; w < W; ++w)
-        t = fmaxf(t, (float)s.d[w]);
-    __syncthreads();
-    return t;
-}
 // (in a fixed order: the lanes of a wave, then the waves)
 template <int W>
 __device__ __forceinline__ double all_sum(double v, Share<W>& s)
