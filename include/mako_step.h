@@ -17,8 +17,9 @@
  * Every pointer inside a descriptor is a DEVICE pointer.  The calls enqueue their kernels on `stream` (a hipStream_t, or null
  * for the default stream) and return without waiting; they allocate nothing, may be captured into a graph, and leave the
  * calling thread's current device as it was.  One call at a time per context: calls on one context, and replays of graphs
- * that hold such calls, must follow each other in stream order, since they share its scratch memory.  Failures are the
- * negative codes of mako_sampler.h.  Results do not depend on the batch a row is in, nor on timing.
+ * that hold such calls, must follow each other in stream order, since they share its scratch memory.  A context outlives the
+ * graphs that hold its calls.  Failures are the negative codes of mako_sampler.h.  Results do not depend on the batch a row is
+ * in, nor on timing.
  */
 #ifndef MAKO_STEP_H
 #define MAKO_STEP_H
