@@ -49,7 +49,12 @@ int fail(mako_step_ctx* ctx, int code, const char* what, const char* more = "")
     snprintf(ctx->err, sizeof ctx->err, "%s%s", what, more);
     return code;
 }
-// Of a call's launches (a failed one is reported by this call, not by the next that looks).
+// Of a call's launches: an error that is there before them is an earlier call's; a failed one is reported by this call, not by the
+// next that looks.
+void launching()
+{
+    (void)hipGetLastError();
+}
 int launched(mako_step_ctx* ctx)
 {
     const hipError_t e = hipGetLastError();
@@ -155,6 +160,7 @@ int mako_step_cut_rows(mako_step_ctx* ctx, const mako_cut_desc* desc, void* stre
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
     hipStream_t st = static_cast<hipStream_t>(stream);
+    launching();
     mako::step::launch_cut(st, d, ctx->sc);
     if (d.out_probs)
         mako::step::launch_probs(st, d);
@@ -173,6 +179,7 @@ int mako_step_verify_drafts(mako_step_ctx* ctx, const mako_verify_desc* desc, vo
     const OnDevice on(ctx->device);
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
+    launching();
     mako::step::launch_verify(static_cast<hipStream_t>(stream), d, ctx->sc);
     return launched(ctx);
 }
@@ -187,6 +194,7 @@ int mako_step_assign_blocks(mako_step_ctx* ctx, const mako_blocks_desc* desc, vo
     const OnDevice on(ctx->device);
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
+    launching();
     mako::step::launch_blocks(static_cast<hipStream_t>(stream), d, ctx->sc);
     return launched(ctx);
 }

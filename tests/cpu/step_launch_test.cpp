@@ -1,0 +1,156 @@
+// What the step's entry points do where launches fail, without a GPU: the HIP functions that they call are this program's (its
+// symbols come before the runtime's), and count the launches.
+#include <dlfcn.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include "../../include/mako_step.h"
+
+namespace {
+struct Dim {
+    uint32_t x, y, z;
+};
+constexpr int kNotReady = 600;  // hipErrorNotReady
+int pending = 0;  // the thread's last error
+int launches = 0;
+int failures = 0;
+
+void expect(const char* call, const char* what, bool ok)
+{
+    if (!ok) {
+        printf("%s: %s\n", call, what);
+        ++failures;
+    }
+}
+} // namespace
+
+extern "C" {
+int hipGetDevice(int* device)
+{
+    *device = 0;
+    return 0;
+}
+int hipSetDevice(int)
+{
+    return 0;
+}
+int hipMalloc(void** p, size_t bytes)
+{
+    *p = malloc(bytes);
+    return *p ? 0 : 2;
+}
+int hipFree(void* p)
+{
+    free(p);
+    return 0;
+}
+int hipFuncSetAttribute(const void*, int, int)
+{
+    return 0;
+}
+int hipGetLastError()
+{
+    const int e = pending;
+    pending = 0;
+    return e;
+}
+int __hipPushCallConfiguration(Dim, Dim, size_t, void*)
+{
+    return 0;
+}
+int __hipPopCallConfiguration(Dim* grid, Dim* block, size_t* lds, void** stream)
+{
+    *grid = *block = {1, 1, 1};
+    *lds = 0;
+    *stream = nullptr;
+    return 0;
+}
+int hipLaunchKernel(const void*, Dim, Dim, void**, size_t, void*)
+{
+    ++launches;
+    return 0;
+}
+}
+
+int main(int, char** argv)
+{
+    void* lib = dlopen(argv[1], RTLD_NOW | RTLD_LOCAL);
+    if (!lib) {
+        printf("%s\n", dlerror());
+        return 1;
+    }
+    const auto create = reinterpret_cast<decltype(&mako_step_create)>(dlsym(lib, "mako_step_create"));
+    const auto destroy = reinterpret_cast<decltype(&mako_step_destroy)>(dlsym(lib, "mako_step_destroy"));
+    const auto cut_rows = reinterpret_cast<decltype(&mako_step_cut_rows)>(dlsym(lib, "mako_step_cut_rows"));
+    const auto verify_drafts = reinterpret_cast<decltype(&mako_step_verify_drafts)>(dlsym(lib, "mako_step_verify_drafts"));
+    const auto assign_blocks = reinterpret_cast<decltype(&mako_step_assign_blocks)>(dlsym(lib, "mako_step_assign_blocks"));
+    mako_step_ctx* ctx = nullptr;
+    if (create(&ctx, 0, 3000, 8192) != MAKO_OK) {
+        printf("no context\n");
+        return 1;
+    }
+    alignas(16) static char memory[64]; // (nothing is read there: no kernel runs)
+    int32_t* const ints = reinterpret_cast<int32_t*>(memory);
+
+    mako_cut_desc cut;
+    memset(&cut, 0, sizeof cut);
+    cut.logits = cut.params = reinterpret_cast<mako_sampling_params*>(memory);
+    cut.out_cuts = reinterpret_cast<mako_row_cut*>(memory);
+    cut.n_rows = 4;
+    cut.n_vocab = 1000;
+    cut.logits_stride = cut.probs_stride = 8192;
+    mako_cut_desc wide = cut, dense;
+    wide.n_vocab = 8192;
+    dense = wide;
+    dense.out_probs = reinterpret_cast<float*>(memory);
+
+    mako_verify_desc verify;
+    memset(&verify, 0, sizeof verify);
+    verify.n_requests = 4;
+    verify.n_vocab = 1000;
+    verify.target = memory;
+    verify.target_stride = 1000;
+    verify.u = reinterpret_cast<float*>(memory);
+    verify.out_tokens = verify.out_accepted = ints;
+
+    mako_blocks_desc blocks;
+    memset(&blocks, 0, sizeof blocks);
+    blocks.n_requests = 4;
+    blocks.block_size = 16;
+    blocks.seq_len = blocks.new_len = ints;
+    blocks.block_table = blocks.free_blocks = blocks.out_start = blocks.out_status = ints;
+    blocks.n_blocks = blocks.n_free = ints;
+    blocks.out_n_blocks = blocks.out_n_free = ints; // (in place)
+    blocks.table_stride = blocks.max_blocks = 8;
+    blocks.free_capacity = 8;
+    blocks.max_tokens = 16;
+    blocks.out_slots = reinterpret_cast<int64_t*>(memory);
+    mako_blocks_desc many_tokens = blocks, many_requests = blocks;
+    many_tokens.max_tokens = 5000;
+    many_requests.n_requests = 3000;
+
+    const auto each = [&](auto f) {
+        f("cut", 2, [&] { return cut_rows(ctx, &cut, nullptr); });
+        f("cut with lists", 4, [&] { return cut_rows(ctx, &wide, nullptr); });
+        f("cut with probabilities", 5, [&] { return cut_rows(ctx, &dense, nullptr); });
+        f("verify", 2, [&] { return verify_drafts(ctx, &verify, nullptr); });
+        f("blocks", 1, [&] { return assign_blocks(ctx, &blocks, nullptr); });
+        f("blocks of many tokens", 2, [&] { return assign_blocks(ctx, &many_tokens, nullptr); });
+        f("blocks of many requests", 2, [&] { return assign_blocks(ctx, &many_requests, nullptr); });
+    };
+    each([&](const char* name, int n, auto call) {
+        launches = 0;
+        expect(name, "fails where nothing does", call() == MAKO_OK && launches == n);
+        // an error of some earlier call, which nobody has looked at yet, is not this call's
+        launches = 0;
+        pending = kNotReady;
+        expect(name, "takes an earlier error for its own", call() == MAKO_OK && launches == n);
+        pending = 0;
+    });
+    destroy(ctx);
+    if (!failures)
+        printf("ok\n");
+    return failures ? 1 : 0;
+}
