@@ -18,7 +18,9 @@
  * for the default stream) and return without waiting; they allocate nothing, may be captured into a graph, and leave the
  * calling thread's current device as it was.  One call at a time per context: calls on one context, and replays of graphs
  * that hold such calls, must follow each other in stream order, since they share its scratch memory.  A context outlives the
- * graphs that hold its calls.  Failures are the negative codes of mako_sampler.h.  Results do not depend on the batch a row is
+ * graphs that hold its calls.  Failures are the negative codes of mako_sampler.h; a call that is refused writes nothing, and behind a
+ * launch that fails (MAKO_ERR_HIP) nothing more is enqueued and what the call's output arrays hold is undefined, those that replace
+ * their inputs too: such a call is repeated from inputs that are known.  Results do not depend on the batch a row is
  * in, nor on timing.
  */
 #ifndef MAKO_STEP_H

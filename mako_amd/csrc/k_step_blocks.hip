@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(256) apply_kernel(mako_blocks_desc d, Scratch 
 
 } // namespace
 
-void launch_blocks(hipStream_t st, const mako_blocks_desc& d, const Scratch& sc)
+hipError_t launch_blocks(hipStream_t st, const mako_blocks_desc& d, const Scratch& sc)
 {
     const uint32_t items = max(d.max_tokens, d.n_requests);
     if (d.n_requests <= kPlanned) {
@@ -283,13 +283,11 @@ void launch_blocks(hipStream_t st, const mako_blocks_desc& d, const Scratch& sc)
         const bool copied = workgroups > 1u && (d.n_blocks == d.out_n_blocks || d.n_free == d.out_n_free);
         int32_t* counts = copied ? reinterpret_cast<int32_t*>(sc.held) : d.out_n_blocks;
         int32_t* n_free = copied ? reinterpret_cast<int32_t*>(sc.free_state) : d.out_n_free;
-        hipLaunchKernelGGL(blocks_kernel, dim3(workgroups), dim3(kThreads), 0, st, d, counts, n_free);
-        if (copied)
-            hipLaunchKernelGGL(counts_kernel, dim3((d.n_requests + 255u) / 256u), dim3(256), 0, st, d, counts, n_free);
-        return;
+        const hipError_t e = launch(blocks_kernel, dim3(workgroups), kThreads, 0, st, d, counts, n_free);
+        return e != hipSuccess || !copied ? e : launch(counts_kernel, dim3((d.n_requests + 255u) / 256u), 256, 0, st, d, counts, n_free);
     }
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, st, d, sc);
-    hipLaunchKernelGGL(apply_kernel, dim3(min((items + 255u) / 256u, 2048u)), dim3(256), 0, st, d, sc);
+    const hipError_t e = launch(plan_kernel, dim3(1), kThreads, 0, st, d, sc);
+    return e != hipSuccess ? e : launch(apply_kernel, dim3(min((items + 255u) / 256u, 2048u)), 256, 0, st, d, sc);
 }
 
 } // namespace step

@@ -1130,19 +1130,23 @@ __global__ void __launch_bounds__(256) probs_kernel(mako_cut_desc d)
 
 constexpr uint32_t kWideWorkgroups = 512; // (two to a CU: what fits; 512 wide rows of 32000 take 75 us in all, with 256 workgroups 82)
 template <class E>
-void cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
-    launch_scan(st, d, sc);
-    hipLaunchKernelGGL(row_kernel<E>, dim3(d.n_rows), dim3(kThreads), sizeof(RowLds), st, d, sc);
+    hipError_t e = launch_scan(st, d, sc);
+    if (e == hipSuccess)
+        e = launch(row_kernel<E>, dim3(d.n_rows), kThreads, sizeof(RowLds), st, d, sc);
     if (d.n_vocab <= kWholeRow)
-        return; // (every row's tokens are listed: its cut is found there)
-    launch_look(st, d, sc);
-    hipLaunchKernelGGL(wide_kernel<E>, dim3(d.n_rows < kWideWorkgroups ? d.n_rows : kWideWorkgroups), dim3(kThreads), sizeof(RowLds), st, d, sc);
+        return e; // (every row's tokens are listed: its cut is found there)
+    if (e == hipSuccess)
+        e = launch_look(st, d, sc);
+    if (e == hipSuccess)
+        e = launch(wide_kernel<E>, dim3(d.n_rows < kWideWorkgroups ? d.n_rows : kWideWorkgroups), kThreads, sizeof(RowLds), st, d, sc);
+    return e;
 }
 template <class E>
-void probs(hipStream_t st, const mako_cut_desc& d)
+hipError_t probs(hipStream_t st, const mako_cut_desc& d)
 {
-    hipLaunchKernelGGL(probs_kernel<E>, dim3((d.n_vocab + kProbs - 1) / kProbs, d.n_rows), dim3(256), 0, st, d);
+    return launch(probs_kernel<E>, dim3((d.n_vocab + kProbs - 1) / kProbs, d.n_rows), 256, 0, st, d);
 }
 
 } // namespace
@@ -1160,14 +1164,14 @@ hipError_t init_cut()
     return hipSuccess;
 }
 
-void launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
-    d.logits_type == MAKO_LOGITS_F32 ? cut<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? cut<BF16>(st, d, sc) : cut<F16>(st, d, sc));
+    return d.logits_type == MAKO_LOGITS_F32 ? cut<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? cut<BF16>(st, d, sc) : cut<F16>(st, d, sc));
 }
 
-void launch_probs(hipStream_t st, const mako_cut_desc& d)
+hipError_t launch_probs(hipStream_t st, const mako_cut_desc& d)
 {
-    d.logits_type == MAKO_LOGITS_F32 ? probs<F32>(st, d) : (d.logits_type == MAKO_LOGITS_BF16 ? probs<BF16>(st, d) : probs<F16>(st, d));
+    return d.logits_type == MAKO_LOGITS_F32 ? probs<F32>(st, d) : (d.logits_type == MAKO_LOGITS_BF16 ? probs<BF16>(st, d) : probs<F16>(st, d));
 }
 
 } // namespace step

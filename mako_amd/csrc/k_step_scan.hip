@@ -258,29 +258,29 @@ __global__ void __launch_bounds__(256, 6) look_kernel(mako_cut_desc d, Scratch s
 }
 
 template <class E>
-void scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
-    hipLaunchKernelGGL(scan_kernel<E>, dim3((chunks_of(d.n_vocab) + 3) / 4, d.n_rows), dim3(256), 0, st, d, sc);
+    return launch(scan_kernel<E>, dim3((chunks_of(d.n_vocab) + 3) / 4, d.n_rows), 256, 0, st, d, sc);
 }
 
 constexpr uint32_t kLookWorkgroups = 4096; // (256 wide rows of 151552 take 111 us in all, with 2048 114, with 8192 112)
 template <class E>
-void look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
     const uint32_t items = d.n_rows * ((chunks_of(d.n_vocab) + 3) / 4); // (65535 rows of 256 at most)
-    hipLaunchKernelGGL(look_kernel<E>, dim3(items < kLookWorkgroups ? items : kLookWorkgroups), dim3(256), 0, st, d, sc);
+    return launch(look_kernel<E>, dim3(items < kLookWorkgroups ? items : kLookWorkgroups), 256, 0, st, d, sc);
 }
 
 } // namespace
 
-void launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
-    d.logits_type == MAKO_LOGITS_F32 ? scan<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? scan<BF16>(st, d, sc) : scan<F16>(st, d, sc));
+    return d.logits_type == MAKO_LOGITS_F32 ? scan<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? scan<BF16>(st, d, sc) : scan<F16>(st, d, sc));
 }
 
-void launch_look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
+hipError_t launch_look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc)
 {
-    d.logits_type == MAKO_LOGITS_F32 ? look<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? look<BF16>(st, d, sc) : look<F16>(st, d, sc));
+    return d.logits_type == MAKO_LOGITS_F32 ? look<F32>(st, d, sc) : (d.logits_type == MAKO_LOGITS_BF16 ? look<BF16>(st, d, sc) : look<F16>(st, d, sc));
 }
 
 } // namespace step

@@ -395,25 +395,25 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
 // 21.1, 7.9 and 16.6 us when with 2048 they took 15.5, 8.0 and 14.7, with 4096 17.0, 12.3 and 15.2)
 constexpr uint32_t kWorkgroups = 2048;
 template <class E, class Q>
-void verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
+hipError_t verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
 {
     const uint32_t parts = (d.n_vocab + kPart - 1) / kPart;
     const uint32_t each = (uint32_t)min((uint64_t)kMostParts, ((uint64_t)parts * d.n_requests + kWorkgroups - 1) / kWorkgroups);
-    hipLaunchKernelGGL((left_kernel<E, Q>), dim3((parts + each - 1) / each, d.n_requests), dim3(kThreads), 0, st, d, sc, each);
-    hipLaunchKernelGGL((draw_kernel<E, Q>), dim3(d.n_requests), dim3(kThreads), 0, st, d, sc);
+    const hipError_t e = launch(left_kernel<E, Q>, dim3((parts + each - 1) / each, d.n_requests), kThreads, 0, st, d, sc, each);
+    return e != hipSuccess ? e : launch(draw_kernel<E, Q>, dim3(d.n_requests), kThreads, 0, st, d, sc);
 }
 template <class E>
-void verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
+hipError_t verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
 {
     const uint32_t q = d.draft ? d.draft_type : d.target_type;
-    q == MAKO_LOGITS_F32 ? verify<E, F32>(st, d, sc) : (q == MAKO_LOGITS_BF16 ? verify<E, BF16>(st, d, sc) : verify<E, F16>(st, d, sc));
+    return q == MAKO_LOGITS_F32 ? verify<E, F32>(st, d, sc) : (q == MAKO_LOGITS_BF16 ? verify<E, BF16>(st, d, sc) : verify<E, F16>(st, d, sc));
 }
 
 } // namespace
 
-void launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
+hipError_t launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
 {
-    d.target_type == MAKO_LOGITS_F32 ? verify<F32>(st, d, sc) : (d.target_type == MAKO_LOGITS_BF16 ? verify<BF16>(st, d, sc) : verify<F16>(st, d, sc));
+    return d.target_type == MAKO_LOGITS_F32 ? verify<F32>(st, d, sc) : (d.target_type == MAKO_LOGITS_BF16 ? verify<BF16>(st, d, sc) : verify<F16>(st, d, sc));
 }
 
 } // namespace step

@@ -49,16 +49,14 @@ int fail(mako_step_ctx* ctx, int code, const char* what, const char* more = "")
     snprintf(ctx->err, sizeof ctx->err, "%s%s", what, more);
     return code;
 }
-// Of a call's launches: an error that is there before them is an earlier call's; a failed one is reported by this call, not by the
-// next that looks.
-void launching()
+// Of a call's launches (by their own statuses: an error that an earlier call left is that call's, and stays; a failed launch is
+// reported by this call, not by the next that looks).
+int launched(mako_step_ctx* ctx, hipError_t e)
 {
+    if (e == hipSuccess)
+        return MAKO_OK;
     (void)hipGetLastError();
-}
-int launched(mako_step_ctx* ctx)
-{
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? MAKO_OK : fail(ctx, MAKO_ERR_HIP, "step: a kernel could not be launched: ", hipGetErrorString(e));
+    return fail(ctx, MAKO_ERR_HIP, "step: a kernel could not be launched: ", hipGetErrorString(e));
 }
 
 template <class T>
@@ -160,11 +158,10 @@ int mako_step_cut_rows(mako_step_ctx* ctx, const mako_cut_desc* desc, void* stre
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
     hipStream_t st = static_cast<hipStream_t>(stream);
-    launching();
-    mako::step::launch_cut(st, d, ctx->sc);
-    if (d.out_probs)
-        mako::step::launch_probs(st, d);
-    return launched(ctx);
+    hipError_t e = mako::step::launch_cut(st, d, ctx->sc);
+    if (e == hipSuccess && d.out_probs)
+        e = mako::step::launch_probs(st, d);
+    return launched(ctx, e);
 }
 
 int mako_step_verify_drafts(mako_step_ctx* ctx, const mako_verify_desc* desc, void* stream)
@@ -179,9 +176,7 @@ int mako_step_verify_drafts(mako_step_ctx* ctx, const mako_verify_desc* desc, vo
     const OnDevice on(ctx->device);
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
-    launching();
-    mako::step::launch_verify(static_cast<hipStream_t>(stream), d, ctx->sc);
-    return launched(ctx);
+    return launched(ctx, mako::step::launch_verify(static_cast<hipStream_t>(stream), d, ctx->sc));
 }
 
 int mako_step_assign_blocks(mako_step_ctx* ctx, const mako_blocks_desc* desc, void* stream)
@@ -194,9 +189,7 @@ int mako_step_assign_blocks(mako_step_ctx* ctx, const mako_blocks_desc* desc, vo
     const OnDevice on(ctx->device);
     if (on.status() != hipSuccess)
         return fail(ctx, MAKO_ERR_HIP, "step: the context's device: ", hipGetErrorString(on.status()));
-    launching();
-    mako::step::launch_blocks(static_cast<hipStream_t>(stream), d, ctx->sc);
-    return launched(ctx);
+    return launched(ctx, mako::step::launch_blocks(static_cast<hipStream_t>(stream), d, ctx->sc));
 }
 
 } // extern "C"

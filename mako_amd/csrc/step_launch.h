@@ -74,12 +74,25 @@ __host__ __device__ inline uint32_t chunks_of(uint32_t n_vocab)
     return (n_vocab + kChunk - 1) / kChunk;
 }
 
-void launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
-void launch_look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
-void launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
-void launch_probs(hipStream_t st, const mako_cut_desc& d);
-void launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc);
-void launch_blocks(hipStream_t st, const mako_blocks_desc& d, const Scratch& sc);
+// A kernel's launch, with its own status.
+template <class T>
+struct Given {
+    using type = T;
+};
+template <class... P>
+hipError_t launch(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t lds, hipStream_t st, typename Given<P>::type... args)
+{
+    void* at[] = {&args...};
+    return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), at, lds, st);
+}
+
+// (of more than one launch, the first that fails is the last: the kernels behind it would work on what it did not write)
+hipError_t launch_scan(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
+hipError_t launch_look(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
+hipError_t launch_cut(hipStream_t st, const mako_cut_desc& d, const Scratch& sc);
+hipError_t launch_probs(hipStream_t st, const mako_cut_desc& d);
+hipError_t launch_verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc);
+hipError_t launch_blocks(hipStream_t st, const mako_blocks_desc& d, const Scratch& sc);
 hipError_t init_cut();
 
 } // namespace step

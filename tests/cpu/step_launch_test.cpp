@@ -12,9 +12,9 @@ namespace {
 struct Dim {
     uint32_t x, y, z;
 };
-constexpr int kNotReady = 600;  // hipErrorNotReady
+constexpr int kNotReady = 600, kOutOfResources = 701; // hipErrorNotReady, hipErrorLaunchOutOfResources
 int pending = 0;  // the thread's last error
-int launches = 0;
+int launches = 0, failing = 0; // the launch that fails, from 1 on
 int failures = 0;
 
 void expect(const char* call, const char* what, bool ok)
@@ -69,8 +69,7 @@ int __hipPopCallConfiguration(Dim* grid, Dim* block, size_t* lds, void** stream)
 }
 int hipLaunchKernel(const void*, Dim, Dim, void**, size_t, void*)
 {
-    ++launches;
-    return 0;
+    return ++launches == failing ? pending = kOutOfResources : 0;
 }
 }
 
@@ -85,6 +84,7 @@ int main(int, char** argv)
     const auto destroy = reinterpret_cast<decltype(&mako_step_destroy)>(dlsym(lib, "mako_step_destroy"));
     const auto cut_rows = reinterpret_cast<decltype(&mako_step_cut_rows)>(dlsym(lib, "mako_step_cut_rows"));
     const auto verify_drafts = reinterpret_cast<decltype(&mako_step_verify_drafts)>(dlsym(lib, "mako_step_verify_drafts"));
+    const auto last_error = reinterpret_cast<decltype(&mako_step_last_error)>(dlsym(lib, "mako_step_last_error"));
     const auto assign_blocks = reinterpret_cast<decltype(&mako_step_assign_blocks)>(dlsym(lib, "mako_step_assign_blocks"));
     mako_step_ctx* ctx = nullptr;
     if (create(&ctx, 0, 3000, 8192) != MAKO_OK) {
@@ -148,6 +148,15 @@ int main(int, char** argv)
         pending = kNotReady;
         expect(name, "takes an earlier error for its own", call() == MAKO_OK && launches == n);
         pending = 0;
+        // a launch that fails is the last, and the call's alone
+        for (failing = 1; failing <= n; ++failing) {
+            launches = 0;
+            expect(name, "does not report a failed launch", call() == MAKO_ERR_HIP && strstr(last_error(ctx), "could not be launched"));
+            expect(name, "goes on behind a failed launch", launches == failing);
+            expect(name, "leaves its error to the next call", pending == 0);
+            pending = 0;
+        }
+        failing = 0;
     });
     destroy(ctx);
     if (!failures)
