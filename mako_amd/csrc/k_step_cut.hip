@@ -133,14 +133,14 @@ __device__ __forceinline__ void add_to_bin(RowLds& lds, uint32_t bin, u64 units)
     atomicAdd(&lds.mass[bin], units);
 }
 
-// The first bin with which the running count and mass get where the cut is, behind `count` tokens that weigh start(units of all
-// in the bins).
+// The first bin with which the running count and mass get where the cut is, behind `count` tokens; what these and some of the bins'
+// tokens weigh is mass(the latter's units, the units of all in the bins).
 struct Bin {
     uint32_t at, before, n; // n 0: none does.  before: tokens in the bins before it
     u64 mass_before, all;   // and their weights' units, and those of all
 };
 template <class E, class F>
-__device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, F start, RowLds& lds)
+__device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uint32_t count, F mass, RowLds& lds)
 {
     const uint32_t a = 2u * threadIdx.x;
     const uint32_t c[2] = {lds.count[a], lds.count[a + 1]};
@@ -163,11 +163,10 @@ __device__ __forceinline__ Bin find_bin(const Row<E>& row, const Want& want, uin
         }
         all += lds.share.u[w];
     }
-    const double mass = start(all);
-    bool was = cb != 0 && want.reached(count + cb, mass + row.mass(mb));
+    bool was = cb != 0 && want.reached(count + cb, mass(mb, all));
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const bool is = want.reached(count + cb + c[k], mass + row.mass(mb + m[k]));
+        const bool is = want.reached(count + cb + c[k], mass(mb + m[k], all));
         if (c[k] != 0 && is && !was) {
             lds.at = a + (uint32_t)k;
             lds.before = cb;
@@ -370,7 +369,7 @@ __device__ __forceinline__ Cut cut_in_bin(const Row<E>& row, const Want& want, c
 template <class E>
 __device__ __forceinline__ Cut cut_in_bins(const Row<E>& row, const Want& want, const Bins& bins, uint32_t n, RowLds& lds)
 {
-    const Bin bin = find_bin(row, want, 0u, [](u64) { return 0.0; }, lds);
+    const Bin bin = find_bin(row, want, 0u, [&](u64 upto, u64) { return row.mass(upto); }, lds);
     if (bin.n == 0)
         return {0, 0.0, 0.0f, 0};
     return cut_in_bin(row, want, bins, bin, n, 0u, 0.0, lds);
@@ -410,7 +409,9 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
         atomicAdd(&lds.mass[kBins - 1u], last_units);
     }
     __syncthreads();
-    Bin bin = find_bin(row, want, 0, [](u64) { return 0.0; }, lds);
+    Bin bin = find_bin(row, want, 0, [&](u64 upto, u64) { return row.mass(upto); }, lds);
+    if (bin.n == 0) // (all the row's tokens, as whole units, weigh less than is wanted of their sum: nothing is cut off)
+        return {tokens, total, 0.0f, 0};
     const uint32_t first = bin.at;
     uint32_t before = bin.before;
     u64 mass_before = bin.mass_before;
@@ -425,7 +426,9 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
                 add_to_bin(lds, (order_key(v) >> next) & ((1u << bits) - 1u), row.units(row.weigh(v)));
         });
         __syncthreads();
-        bin = find_bin(row, want, before, [&](u64) { return row.mass(mass_before); }, lds);
+        // (one of them: what weighs enough up to the end of the bin that is divided does so up to the last of its parts, since both are
+        // the same whole number of units, made a mass once.  As a sum of two masses it can be a bit less)
+        bin = find_bin(row, want, before, [&](u64 upto, u64) { return row.mass(mass_before + upto); }, lds);
         prefix = (shift == 32u ? 0u : prefix << bits) | bin.at;
         before += bin.before;
         mass_before += bin.mass_before;
@@ -1002,7 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
                 list_bins = Bins(from, from - low);
                 bin_list(row, list_bins, n, lds);
                 auto before = [&](u64 all) { return plan.from_above ? side : total - side - row.mass(all); };
-                const Bin bin = find_bin(row, want, above, before, lds);
+                const Bin bin = find_bin(row, want, above, [&](u64 upto, u64 all) { return before(all) + row.mass(upto); }, lds);
                 if (above && want.reached(above, before(bin.all))) {
                     const float width = from - low;
                     low = high;
@@ -1043,7 +1046,7 @@ __global__ void __launch_bounds__(kThreads, 4) wide_kernel(mako_cut_desc d, Scra
                     const float from = fminf(high, row.max);
                     list_bins = Bins(from, from - low);
                     bin_list(row, list_bins, n, lds);
-                    const Bin bin = find_bin(row, want, above, [&](u64) { return weight_above; }, lds);
+                    const Bin bin = find_bin(row, want, above, [&](u64 upto, u64) { return weight_above + row.mass(upto); }, lds);
                     if (bin.n && !(above && want.reached(above, weight_above))) {
                         cut = cut_in_bin(row, want, list_bins, bin, n, above, weight_above, lds);
                         listed_n = n;
