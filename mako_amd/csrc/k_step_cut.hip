@@ -865,8 +865,10 @@ __global__ void __launch_bounds__(kThreads, 4) row_kernel(mako_cut_desc d, Scrat
     row.set_unit(kind.sums ? c.total : (double)max(n_listed, 1u));
     // (a list of all the row's tokens: the bins go as far down as weights matter)
     const Bins bins(row.max, c.listed > -INFINITY ? row.max - c.listed : (float)(64.0 / row.scale));
-    uint32_t rank = kind.top_k ? min(c.count, kind.top_k) : c.count;
-    bool all_weighty = !kind.min_p; // (or it is known how many are)
+    // (no token weighs more than the first, which weighs 1)
+    const bool none_weighty = kind.min_p && p.min_p > 1.0f;
+    uint32_t rank = none_weighty ? 1u : (kind.top_k ? min(c.count, kind.top_k) : c.count);
+    bool all_weighty = none_weighty || !kind.min_p; // (or it is known how many are)
     if (list_there) {
         bin_list(row, bins, n_listed, lds);
         if (kind.min_p) {
