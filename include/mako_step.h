@@ -42,8 +42,9 @@ extern "C" {
 typedef struct mako_step_ctx mako_step_ctx;
 
 /* Creates a context on HIP device `device` for rows (requests) of up to max_rows and vocabularies of up to max_vocab
- * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB); its scratch memory (some 2.5 bytes for every logit of
- * the largest batch, and 160 a row) is allocated here. */
+ * (at most MAKO_STEP_MAX_ROWS and MAKO_STEP_MAX_VOCAB).  Its scratch memory is allocated here: for every row 160 bytes, 8 for each
+ * 1024 of its logits, or part of them, and 32 for each 2048, or 5152 (some 2.5 a logit) with a max_vocab above 6144 (what
+ * mako_step_cut_rows writes there: a context that never cuts rows has it too). */
 #define MAKO_STEP_MAX_ROWS 65535
 #define MAKO_STEP_MAX_VOCAB 1048576
 int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_t max_vocab);

@@ -9,6 +9,7 @@
 #include "../../include/mako_step.h"
 #include "step_checks.h"
 #include "step_common.h"
+#include "step_cut.h"
 #include "step_launch.h"
 
 struct mako_step_ctx {
@@ -90,9 +91,10 @@ int mako_step_create(mako_step_ctx** out, int device, uint32_t max_rows, uint32_
     hipError_t e = on.status();
     if (e == hipSuccess)
         e = take(sc.chunks, rows * sc.chunks_cap);
-    if (e == hipSuccess)
+    const bool lists = max_vocab > mako::step::kWholeRow; // (rows that are held whole have none)
+    if (e == hipSuccess && lists)
         e = take(sc.lists, rows * sc.chunks_cap * mako::step::kChunkList);
-    if (e == hipSuccess)
+    if (e == hipSuccess && lists)
         e = take(sc.looks, rows * sc.chunks_cap * mako::step::kLookList);
     if (e == hipSuccess)
         e = take(sc.plans, rows);

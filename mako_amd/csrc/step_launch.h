@@ -54,7 +54,8 @@ struct Stop {
 
 struct Scratch {
     ChunkRec* chunks;     // [rows][chunks_cap]
-    uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that
+    uint64_t* lists;      // [rows][chunks_cap][kChunkList]: a token's number, and its logit above that (null, like looks, where no row
+                          // is longer than what is held whole)
     uint64_t* looks;      // [rows][chunks_cap][kLookList]: by plan (and the chunks too, then)
     uint32_t chunks_cap;  // of a row
     RowPlan* plans;       // [rows]: of those that have one, in no order

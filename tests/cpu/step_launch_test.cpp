@@ -6,6 +6,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <utility>
+
 #include "../../include/mako_step.h"
 
 namespace {
@@ -15,6 +17,7 @@ struct Dim {
 constexpr int kNotReady = 600, kOutOfResources = 701; // hipErrorNotReady, hipErrorLaunchOutOfResources
 int pending = 0;  // the thread's last error
 int launches = 0, failing = 0; // the launch that fails, from 1 on
+uint64_t allocated = 0, most = ~0ull; // bytes, and how many there are
 int failures = 0;
 
 void expect(const char* call, const char* what, bool ok)
@@ -38,8 +41,9 @@ int hipSetDevice(int)
 }
 int hipMalloc(void** p, size_t bytes)
 {
-    *p = malloc(bytes);
-    return *p ? 0 : 2;
+    *p = bytes <= most - allocated ? malloc(bytes) : nullptr;
+    allocated += *p ? bytes : 0;
+    return *p ? 0 : pending = 2; // hipErrorOutOfMemory
 }
 int hipFree(void* p)
 {
@@ -87,6 +91,23 @@ int main(int, char** argv)
     const auto last_error = reinterpret_cast<decltype(&mako_step_last_error)>(dlsym(lib, "mako_step_last_error"));
     const auto assign_blocks = reinterpret_cast<decltype(&mako_step_assign_blocks)>(dlsym(lib, "mako_step_assign_blocks"));
     mako_step_ctx* ctx = nullptr;
+    // a context's memory is what the header says, whole or not at all
+    const auto parts = [](uint64_t vocab, uint64_t of) { return (vocab + of - 1) / of; };
+    for (const auto& size : {std::pair<uint32_t, uint32_t>{65535, 1}, {65535, 6144}, {3, 6145}, {500, 129280}, {1, 1048576}}) {
+        const uint64_t rows = size.first, bytes = rows * (160 + parts(size.second, 1024) * 8 + parts(size.second, 2048) * (size.second > 6144 ? 5152 : 32));
+        char name[64];
+        snprintf(name, sizeof name, "context for %u rows of %u", size.first, size.second);
+        allocated = 0;
+        expect(name, "fails", create(&ctx, 0, size.first, size.second) == MAKO_OK && ctx);
+        if (allocated < bytes || allocated > bytes + 64) // (a few words of the batch)
+            printf("%llu bytes, expected %llu\n", (unsigned long long)allocated, (unsigned long long)bytes);
+        expect(name, "memory", allocated >= bytes && allocated <= bytes + 64);
+        destroy(ctx);
+        allocated = 0;
+        most = bytes - 1;
+        expect(name, "with too little memory", create(&ctx, 0, size.first, size.second) == MAKO_ERR_NO_MEMORY && !ctx && pending == 0);
+        most = ~0ull;
+    }
     if (create(&ctx, 0, 3000, 8192) != MAKO_OK) {
         printf("no context\n");
         return 1;
