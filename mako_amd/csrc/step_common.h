@@ -152,24 +152,24 @@ __device__ __forceinline__ float key_logit(uint32_t k)
     return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
-// 2^t for t <= 0: 2^round(t) times a polynomial in the rest, of degree 9, the one whose largest relative error over
-// [-1/2, 1/2] is least (found by exchange) with its constant term made 1: 2.7e-14 (degree 10: 2e-16, and an operation more for
-// each logit).  2^0 is exactly 1.  0 below 2^-1074.  kFinite: t is neither NaN nor -infinity.
+// 2^t for t <= 0: 2^round(t) times a polynomial in the rest, of degree 9: of those with a constant term of 1 the one whose largest
+// relative error over [-1/2, 1/2] is least (found by exchange), 1.6e-14 with its roundings (degree 10: 2e-16, and an operation more
+// for each logit).  2^0 is exactly 1.  0 below 2^-1074.  kFinite: t is neither NaN nor -infinity.
 template <bool kFinite = false>
 __device__ __forceinline__ double exp2_down(double t)
 {
     if (!kFinite)
         t = fmax(t, -1100.0);
     const double n = rint(t), f = t - n;
-    double p = 1.0150344092361341e-07;
-    p = fma(p, f, 1.325940551832952e-06);
-    p = fma(p, f, 1.5252984798658376e-05);
-    p = fma(p, f, 0.0001540343494852222);
-    p = fma(p, f, 0.0013333557617675399);
-    p = fma(p, f, 0.0096181291920665896);
-    p = fma(p, f, 0.055504108668685152);
-    p = fma(p, f, 0.24022650695649655);
-    p = fma(p, f, 0.69314718055987101);
+    double p = 1.0148340794092651e-07;
+    p = fma(p, f, 1.3258335415197215e-06);
+    p = fma(p, f, 1.5252990014502824e-05);
+    p = fma(p, f, 0.0001540344088440716);
+    p = fma(p, f, 0.001333355762547261);
+    p = fma(p, f, 0.009618129181163993);
+    p = fma(p, f, 0.05550410866841572);
+    p = fma(p, f, 0.2402265069572282);
+    p = fma(p, f, 0.6931471805598851);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
 }
@@ -178,8 +178,8 @@ __device__ __forceinline__ double exp2_down(double t)
 template <int N>
 __device__ __forceinline__ void exp2_down(const double* t, double* out)
 {
-    constexpr double c[10] = {1.0150344092361341e-07, 1.325940551832952e-06, 1.5252984798658376e-05, 0.0001540343494852222, 0.0013333557617675399,
-                              0.0096181291920665896, 0.055504108668685152, 0.24022650695649655, 0.69314718055987101, 1.0};
+    constexpr double c[10] = {1.0148340794092651e-07, 1.3258335415197215e-06, 1.5252990014502824e-05, 0.0001540344088440716, 0.001333355762547261,
+                              0.009618129181163993, 0.05550410866841572, 0.2402265069572282, 0.6931471805598851, 1.0};
     double n[N], f[N], p[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
