@@ -60,7 +60,7 @@ struct Gate { // of a wave, or of all
 };
 struct Group {
     std::vector<ucontext_t> threads;
-    std::vector<char> stacks, ended;
+    std::vector<char> ended;
     std::vector<Gate> waves;
     Gate all;
     ucontext_t main;
@@ -69,6 +69,8 @@ struct Group {
     void* arg = nullptr;
 };
 inline Group* group = nullptr;
+inline std::vector<char> stacks; // (kept from one workgroup to the next)
+inline bool backwards = false;   // the last thread first: what a barrier is missing for is seen by one of the orders
 
 inline void yield()
 {
@@ -104,7 +106,8 @@ void run(uint32_t threads, F body)
     Group g;
     group = &g;
     g.threads.resize(threads);
-    g.stacks.resize(threads * kStack);
+    if (stacks.size() < threads * kStack)
+        stacks.resize(threads * kStack);
     g.ended.assign(threads, 0);
     g.waves.resize((threads + 63) / 64);
     g.all.members = threads;
@@ -114,20 +117,22 @@ void run(uint32_t threads, F body)
     for (uint32_t t = 0; t < threads; ++t) {
         ++g.waves[t / 64].members;
         getcontext(&g.threads[t]);
-        g.threads[t].uc_stack.ss_sp = g.stacks.data() + t * kStack;
+        g.threads[t].uc_stack.ss_sp = stacks.data() + t * kStack;
         g.threads[t].uc_stack.ss_size = kStack;
         g.threads[t].uc_link = nullptr;
         makecontext(&g.threads[t], entry, 0);
     }
     for (bool any = true; any;) {
         any = false;
-        for (uint32_t t = 0; t < threads; ++t)
+        for (uint32_t i = 0; i < threads; ++i) {
+            const uint32_t t = backwards ? threads - 1 - i : i;
             if (!g.ended[t]) {
                 any = true;
                 g.running = t;
                 threadIdx.x = t;
                 swapcontext(&g.main, &g.threads[t]);
             }
+        }
     }
     group = nullptr;
 }

@@ -107,7 +107,7 @@ int main()
         const Want want = {0, row.mass(before + in)};
         if (row.mass(before) + row.mass(in) >= want.mass)
             continue;
-        ++at_the_end;
+        lanes::backwards = ++at_the_end % 2 == 0;
         expect("mass at a bin's end", seed, g.divide(want), n, last);
     }
     if (at_the_end < 6) {
