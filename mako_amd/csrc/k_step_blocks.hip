@@ -9,7 +9,7 @@
 // Three running sums over the requests (blocks given back, blocks asked for, tokens), and where there is not enough of something
 // a second round of sums over those that are still served.  Every output entry then finds its request in them by halving, 11 steps in
 // LDS, so that the work is even however lengths differ.  Bound by the launch and a handful of trips to memory: 64 requests of five
-// tokens take 4.6 us, 1024 requests with 131072 tokens 8.1 (one plan in device memory and a launch for each half: 10.6 and 18.6),
+// tokens take 4.6 us, 1024 requests with 131072 tokens 7.9 (one plan in device memory and a launch for each half: 10.6 and 18.6),
 // 2048 requests of four tokens 8.8, 2049, whose plan is in device memory, 12.6 to 15.3.
 #include "step_common.h"
 #include "step_launch.h"

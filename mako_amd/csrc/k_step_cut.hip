@@ -15,9 +15,9 @@
 // 1024 bins of logits say which bin holds it, and the bin's tokens are counted against each other.  Weights are 64-bit floats, and
 // where they are added up in an order that chance makes (bins, atomics) whole numbers of a unit, so that results do not vary.
 //
-// What bounds them: 64 rows of 129280 fp32 logits (33.1 MB), some cut beyond their lists, take 44 us: scan 12.7 (2.6 TB/s), row 13.7,
-// look 7.9, wide 10.2; one row of 151552 34: 5.4, 12.8, 7.4, 9.3; 256 of them, half of them flat, 97: 42 (3.7 TB/s, vector
-// instructions 78 % of the time), 15, 24 (6.4 TB/s, from the Infinity Cache) and 15.  row_kernel and wide_kernel are chains of some
+// What bounds them: 64 rows of 129280 fp32 logits (33.1 MB), some cut beyond their lists, take 43 us: scan 12.9 (2.6 TB/s), row 13.9,
+// look 8.0, wide 10.4; one row of 151552 34: 5.4, 12.5, 7.4, 9.0; 256 of them, half of them flat, 96: 42 (3.7 TB/s, vector
+// instructions 78 % of the time), 15, 24 (6.4 TB/s, from the Infinity Cache) and 14.5.  row_kernel and wide_kernel are chains of some
 // fifteen trips to memory, LDS and barriers with one workgroup's latency in each, their code read from memory as they go (a pass
 // fewer through the list, with the exponentials in more places, took 1 us longer).
 #include "step_common.h"
@@ -477,7 +477,7 @@ __device__ __forceinline__ Cut cut_by_division(Row<E>& row, const Want& want, do
 }
 
 // A guess where the cut of a row lies, by a sample of it, an eighth of every chunk in kPieces places (128 bytes of fp32 each): within
-// four deviations, and where these hold too many tokens, within three, or two and a half.  (7 of row_kernel's 12.8 us on one row of 151552, 4 of them
+// four deviations, and where these hold too many tokens, within three, or two and a half.  (7 of row_kernel's 12.5 us on one row of 151552, 4 of them
 // the sample; a sixteenth took as long, with longer lists for wide_kernel.  In one place the times are the same, but rows whose
 // tokens stand in order are guessed wrongly and divided: 290 us instead of 76.)
 // (range: of logits, from the largest down, in which the cut is to be expected; total: not where the cut is by rank)

@@ -7,8 +7,8 @@
 // Of a request's rows only one is read whole, the one behind the last accepted draft, and of the drafter's the one beside it: which
 // these are follows from one logit of each row, which every workgroup looks up for itself (a launch of its own would cost more).
 // What is left, max(0, p - q), is needed as a sum before a token can be drawn by it: the parts' sums first, then one part again.
-// 64 requests over 129280 bf16 logits of each kind (33 MB) take 14.1 and 5.0 us, one over 151552 fp32 logits 5.6 and 4.4, 32 with
-// looked-up drafts under masks 7.4 and 5.1, 256 over 32000 probabilities (66 MB) 11.7 and 4.5: large ones are bound by
+// 64 requests over 129280 bf16 logits of each kind (33 MB) take 14.6 and 5.0 us, one over 151552 fp32 logits 5.6 and 4.4, 32 with
+// looked-up drafts under masks 7.6 and 5.1, 256 over 32000 probabilities (66 MB) 12.6 and 4.6: large ones are bound by
 // memory and the weights' arithmetic (two weights of 20 instructions a token), small ones by five trips to memory in a row, draw_kernel
 // always.
 #include "step_common.h"
@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(kThreads) draw_kernel(mako_verify_desc d, Scra
     }
 }
 
-// (as many as run at a time.  More find the place anew, fewer wait longer for their loads: with 1024 the three larger calls above took
-// 21.1, 7.9 and 16.6 us when with 2048 they took 15.5, 8.0 and 14.7, with 4096 17.0, 12.3 and 15.2)
+// (as many as run at a time.  More find the place anew, fewer wait longer for their loads: with 1024 the three larger calls above take
+// 21.4, 7.7 and 12.8 us, with 2048 14.7, 7.6 and 12.6, with 4096 16.1, 10.2 and 12.6)
 constexpr uint32_t kWorkgroups = 2048;
 template <class E, class Q>
 hipError_t verify(hipStream_t st, const mako_verify_desc& d, const Scratch& sc)
